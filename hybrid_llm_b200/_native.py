@@ -126,6 +126,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     # router local context
     "llmyb_router_ctx_prefill": (I32, [P, I32, I32, I32, I32, P, P, P, P, P]),
     "llmyb_router_ctx_step": (I32, [P, I32, I32, I32, P, P, P, P, P, P]),
+    # paged key-value cache
+    "llmyb_paged_append": (I32, [P, I64, I64, P, I64, I64, P, I64, I64, I32, I32, I32, I32, I32, P,
+                                 P, I64, I64, I64, I32, I32, P, I64, I32, P, P, I32, P, P, F32, P,
+                                 I32, I32, P, I64, I64, P, P]),
+    "llmyb_paged_decode_scratch_bytes": (I64, [I32, I32, I32]),
+    "llmyb_paged_decode": (I32, [P, I64, I64, I32, I32, I32, I32, I32, P, P, I64, I64, I64, I32,
+                                 I32, P, I64, I32, P, F32, F32, I32, P, P, I64, I64, P, P, P, P]),
+    "llmyb_paged_prefill_scratch_bytes": (I64, [I32, I32, I32, I32, I32, I32]),
+    "llmyb_paged_prefill": (I32, [P, I64, I64, I32, I32, I32, I32, I32, P, P, I64, I64, I64, I32,
+                                  I32, P, I64, I32, P, P, I32, P, F32, F32, I32, P, P, I64, I64, P,
+                                  P, P, P]),
 }
 
 _lock = threading.Lock()

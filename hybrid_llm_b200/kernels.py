@@ -1172,3 +1172,200 @@ def csa_remote_step(x: torch.Tensor, q: torch.Tensor, w_comp: torch.Tensor, rati
                  _ptr(_inplace(pend_cnt, "pend_cnt")), _ptr(scratch[0]), _ptr(scratch[1]),
                  _ptr(out), out.stride(0), _ptr(device_status(x.device)), _stream())
     return out
+
+
+# ------------------------------------------------------ paged key-value cache
+PAGE_SIZES = (16, 32, 64, 128, 256)
+_PAGED_DTYPES = (torch.bfloat16, torch.float16)
+
+
+def _paged_rows(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
+    """[N, heads, head_dim] rows of the cache's type."""
+    if t.dim() != 3 or t.dtype != like.dtype or t.shape[2] != like.shape[3]:
+        raise ValueError(f"{name} must be [tokens, heads, {like.shape[3]}] {like.dtype}")
+    sn, sh, sd = t.stride()
+    if sd != 1 or sn % 8 or sh % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{name}: contiguous head dimension, 16-byte aligned rows and heads")
+
+
+def _paged_i32(t: torch.Tensor, name: str, n: int) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.stride(0) != 1:
+        raise ValueError(f"{name} must be contiguous int32 [{n}]")
+
+
+def _paged_f32(t: torch.Tensor | None, name: str, n: int | None = None) -> None:
+    if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or not t.is_contiguous()
+                          or (n is not None and t.shape[0] != n)):
+        raise ValueError(f"{name} must be contiguous fp32" + ("" if n is None else f" [{n}]"))
+
+
+def _paged_pool(k_pages, v_pages, block_table, lengths, *others):
+    """Checks the cache and the devices; returns the pool's ABI arguments."""
+    dev = torch.cuda.current_device() if k_pages.is_cuda else -1
+    for t in (k_pages, v_pages, block_table, lengths, *others):
+        if t is not None and t.get_device() != dev or dev < 0:
+            if t is not None and t.is_cuda and dev >= 0:
+                raise ValueError("paged cache tensors must be on the current CUDA device")
+            raise RuntimeError("llmyb kernels take CUDA tensors only (no CPU fallback)")
+    if (k_pages.dim() != 4 or k_pages.dtype not in _PAGED_DTYPES or k_pages.shape != v_pages.shape
+            or v_pages.dtype != k_pages.dtype or k_pages.stride() != v_pages.stride()):
+        raise ValueError("k_pages and v_pages must be alike: [pages, kv_heads, page_size, head_dim] "
+                         "bf16 or fp16 with the same strides")
+    pages, _, page_size, dim = k_pages.shape
+    sp, sh, sr, sd = k_pages.stride()
+    if page_size not in PAGE_SIZES or dim not in (64, 128):
+        raise ValueError(f"pages of {PAGE_SIZES} rows and head dimensions 64 or 128 are served")
+    if sd != 1 or sp % 8 or sh % 8 or sr % 8 or k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16:
+        raise ValueError("pages: contiguous head dimension, 16-byte aligned pages, heads and rows")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (
+            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table must be int32 [batch, pages per sequence]")
+    _paged_i32(lengths, "lengths", block_table.shape[0])
+    return (sp, sh, sr, pages, page_size, block_table.data_ptr(), block_table.stride(0),
+            block_table.shape[1], lengths.data_ptr())
+
+
+def _paged_out(out, like: torch.Tensor, name: str = "out") -> torch.Tensor:
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if out.shape != like.shape or out.dtype != like.dtype:
+        raise ValueError(f"{name} must have the shape and type of q")
+    sn, sh, sd = out.stride()
+    if sd != 1 or sn % 8 or sh % 8 or out.data_ptr() % 16:
+        raise ValueError(f"{name}: contiguous head dimension, 16-byte aligned rows and heads")
+    return out
+
+
+def _paged_lse(lse, like: torch.Tensor) -> None:
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != like.shape[:2]
+                            or not lse.is_contiguous()):
+        raise ValueError("lse must be contiguous fp32 [tokens, heads]")
+
+
+def _paged_scores(q, k_pages, scale, softcap, window, slopes) -> float:
+    if q.shape[1] % k_pages.shape[1]:
+        raise ValueError("query heads must be a multiple of the kv heads")
+    if not softcap >= 0.0 or window < 0:
+        raise ValueError("softcap and window must be >= 0 (0: none)")
+    _paged_f32(slopes, "slopes", q.shape[1])
+    scale = k_pages.shape[3] ** -0.5 if scale is None else float(scale)
+    if not scale > 0.0:
+        raise ValueError("scale must be positive")
+    return scale
+
+
+def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
+                 v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, *,
+                 cu_q: torch.Tensor | None = None, inv_freq: torch.Tensor | None = None,
+                 interleaved: bool = False, q_norm: torch.Tensor | None = None,
+                 k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                 q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """New tokens into a paged key-value cache; returns the queries to attend with.
+
+    q [N, Hq, Dh], k and v [N, Hkv, Dh] (column slices of a fused projection
+    are fine) get an RMS norm per head (q_norm / k_norm fp32 [Dh]) and rotary
+    positions (inv_freq fp32 [R/2]: the first R dimensions of a head turn by
+    position * inv_freq, in half-split or interleaved pairs); k and v are
+    stored in k_pages / v_pages [pages, Hkv, page_size, Dh] (any page, head and
+    row strides) at block_table [B, W] int32.  lengths [B] int32 count the new
+    tokens too: tokens cu_q[b] .. cu_q[b+1) (int32 [B+1]; None: one per
+    sequence) are the last positions of sequence b.  Rows behind cu_q[B] are
+    left alone; a token at a negative position (a slot of length 0) is not
+    stored and its query is zero.  q_out may be q."""
+    pool = _paged_pool(k_pages, v_pages, block_table, lengths, q, k, v, cu_q, inv_freq, q_norm,
+                       k_norm, q_out)
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        _paged_rows(t, name, k_pages)
+    n, heads, dim = q.shape
+    kv = k_pages.shape[1]
+    if k.shape != (n, kv, dim) or v.shape != (n, kv, dim):
+        raise ValueError(f"k and v must be [{n}, {kv}, {dim}]")
+    batch = lengths.shape[0]
+    if cu_q is not None:
+        _paged_i32(cu_q, "cu_q", batch + 1)
+    elif n != batch:
+        raise ValueError("without cu_q there is one token per sequence")
+    _paged_f32(q_norm, "q_norm", dim)
+    _paged_f32(k_norm, "k_norm", dim)
+    _paged_f32(inv_freq, "inv_freq")
+    half = 0 if inv_freq is None else inv_freq.shape[0]
+    if half % 8 or 2 * half > dim:
+        raise ValueError(f"inv_freq must have a multiple of 8 values, at most {dim // 2}")
+    q_out = _paged_out(q_out, q, "q_out")
+    _native.call("llmyb_paged_append", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
+                 k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), n, heads, kv,
+                 dim, k_pages.dtype is torch.float16, k_pages.data_ptr(), v_pages.data_ptr(),
+                 *pool, _ptr(cu_q), batch, _ptr(q_norm), _ptr(k_norm), eps, _ptr(inv_freq), half,
+                 interleaved, q_out.data_ptr(), q_out.stride(0), q_out.stride(1),
+                 device_status(q.device).data_ptr(), _stream())
+    return q_out
+
+
+def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 block_table: torch.Tensor, lengths: torch.Tensor, *, scale: float | None = None,
+                 softcap: float = 0.0, window: int = 0, slopes: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one token per sequence (q [B, Hq, Dh], the last position of
+    each) over a paged cache (see paged_append) -> [B, Hq, Dh].
+
+    Scores scale * q.k (scale Dh^-0.5), softcap * tanh(s / softcap) if softcap,
+    minus slopes[h] * distance if slopes (fp32 [Hq]); window > 0 keeps the keys
+    at distance < window.  Query head h reads kv head h // (Hq / Hkv).  A
+    sequence of length 0 gives zeros.  lse (fp32 [B, Hq]) receives the natural
+    log-sum-exp of the scores."""
+    pool = _paged_pool(k_pages, v_pages, block_table, lengths, q, slopes, out, lse)
+    _paged_rows(q, "q", k_pages)
+    b, heads, dim = q.shape
+    kv = k_pages.shape[1]
+    if b != lengths.shape[0]:
+        raise ValueError("q must have one row per sequence of block_table")
+    scale = _paged_scores(q, k_pages, scale, softcap, window, slopes)
+    out = _paged_out(out, q)
+    _paged_lse(lse, q)
+    need = _native.lib().llmyb_paged_decode_scratch_bytes(heads, kv, dim)
+    scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _native.call("llmyb_paged_decode", q.data_ptr(), q.stride(0), q.stride(1), b, heads, kv, dim,
+                 k_pages.dtype is torch.float16, k_pages.data_ptr(), v_pages.data_ptr(), *pool,
+                 scale, softcap, window, _ptr(slopes), out.data_ptr(), out.stride(0),
+                 out.stride(1), _ptr(lse), scratch.data_ptr(), device_status(q.device).data_ptr(),
+                 _stream())
+    return out
+
+
+def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                  block_table: torch.Tensor, lengths: torch.Tensor, cu_q: torch.Tensor, *,
+                  scale: float | None = None, softcap: float = 0.0, window: int = 0,
+                  slopes: torch.Tensor | None = None, prefix: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of several new tokens per sequence over a paged cache that
+    already holds them (see paged_append) -> [N, Hq, Dh].
+
+    q [N, Hq, Dh] packed by cu_q; scores as in paged_decode.  A token at
+    position i sees the keys j <= i of its own sequence with i - j < window
+    (window > 0) or, instead of a window, also those j < prefix[b] (int32 [B]:
+    a bidirectional prefix).  Rows that see no key give zeros; rows behind
+    cu_q[B] are left alone.  lse: fp32 [N, Hq]."""
+    pool = _paged_pool(k_pages, v_pages, block_table, lengths, q, cu_q, slopes, prefix, out, lse)
+    _paged_rows(q, "q", k_pages)
+    n, heads, dim = q.shape
+    kv = k_pages.shape[1]
+    batch = lengths.shape[0]
+    _paged_i32(cu_q, "cu_q", batch + 1)
+    scale = _paged_scores(q, k_pages, scale, softcap, window, slopes)
+    if heads // kv > 128:
+        raise ValueError("at most 128 query heads per kv head")
+    if prefix is not None:
+        _paged_i32(prefix, "prefix", batch)
+        if window:
+            raise ValueError("a prefix and a window exclude each other")
+    out = _paged_out(out, q)
+    _paged_lse(lse, q)
+    need = _native.lib().llmyb_paged_prefill_scratch_bytes(n, heads, kv, dim, block_table.shape[1],
+                                                           k_pages.shape[2])
+    scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _native.call("llmyb_paged_prefill", q.data_ptr(), q.stride(0), q.stride(1), n, heads, kv, dim,
+                 k_pages.dtype is torch.float16, k_pages.data_ptr(), v_pages.data_ptr(), *pool,
+                 cu_q.data_ptr(), batch, _ptr(prefix), scale, softcap, window, _ptr(slopes),
+                 out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse), _ptr(scratch),
+                 device_status(q.device).data_ptr(), _stream())
+    return out

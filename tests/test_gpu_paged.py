@@ -1,0 +1,529 @@
+"""GPU: paged key-value cache (append, decode, prefill) against the float64 oracle.
+
+Tolerances, derived from the arithmetic.  u = half a step of the type relative
+to the value (bf16 2^-8, fp16 2^-11).
+  append     fp32 throughout, one rounding: u |x| + 2e-6 (|a| + |b|); the second
+             term bounds the angle's rounding to 32 bits after its reduction
+             (2^-23 pi), the sine's and the norm's few 2^-24
+  attention  the output's rounding u |out|, plus the weights' rounding to the
+             cache's type: u sum p|v| (each weight off by at most u of itself),
+             plus 2^-12 sum p|v| for the fp32 products and exponentials (scores
+             off by at most 2^-13: D 2^-24 sum |q k| scale < 128 2^-24 10), plus
+             for fp16 n 2^-25 max|v| (weights below 2^-14 are subnormal)
+  lse        2^-13 (the scores) + 2^-20 |lse|
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+class Cache:
+    """Pages of random rows; every slot that no sequence holds is NaN or infinite."""
+
+    def __init__(self, lengths, kv, dim, page, dtype, seed, layout="hnd", spare=3, pad=2):
+        rng = np.random.default_rng(seed)
+        need = [-(-n // page) for n in lengths]
+        self.pages = sum(need) + spare
+        width = max(need + [0]) + pad
+        order = rng.permutation(self.pages).astype(np.int32)
+        self.table = np.full((len(lengths), width), -1, np.int32)
+        at = 0
+        for b, n in enumerate(need):
+            self.table[b, :n] = order[at:at + n]
+            at += n
+        shape = (self.pages, kv, page, dim)
+        self.k = torch.from_numpy(rng.normal(size=shape).astype(np.float32)).to(dtype)
+        self.v = torch.from_numpy(rng.normal(size=shape).astype(np.float32)).to(dtype)
+        held = np.zeros((self.pages, page), bool)
+        for b, n in enumerate(lengths):
+            p = np.arange(n)
+            held[self.table[b, p // page], p % page] = True
+        bad = torch.from_numpy(~held)[:, None, :, None].expand(shape)
+        poison = torch.tensor([float("nan"), float("inf"), -float("inf")], dtype=dtype)
+        poison = poison[torch.arange(self.k.numel()).reshape(shape) % 3]
+        self.k = torch.where(bad, poison, self.k)
+        self.v = torch.where(bad, poison, self.v)
+        self.k_ref = np.where(_np(bad) > 0, 0.0, _np(self.k))
+        self.v_ref = np.where(_np(bad) > 0, 0.0, _np(self.v))
+        self.kd, self.vd = self.k.cuda(), self.v.cuda()
+        if layout == "nhd":  # [page, row, head, dim] memory
+            self.kd, self.vd = (t.transpose(1, 2).contiguous().transpose(1, 2)
+                                for t in (self.kd, self.vd))
+        self.lengths = np.asarray(lengths, np.int32)
+        self.td = torch.from_numpy(self.table).cuda()
+        self.ld = torch.from_numpy(self.lengths).cuda()
+
+
+def _close(got, ref, mag, dtype, lens, vmax):
+    u = U[dtype]
+    tol = u * np.abs(ref) + (u + 2.0 ** -12) * mag
+    if dtype is torch.float16:
+        tol = tol + max(lens) * 2.0 ** -25 * vmax
+    bad = ~(np.abs(_np(got) - ref) <= tol)
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:5], np.abs(_np(got) - ref).max())
+
+
+def _check(out, lse, cache, q, cu, dtype, **kw):
+    dim = q.shape[-1]
+    kw.setdefault("scale", dim ** -0.5)
+    ref, mag, l_ref = paged.attention(_np(q), cache.k_ref, cache.v_ref, cache.table, cache.lengths,
+                                      cu, **kw)
+    n = cu[-1]
+    _close(out[:n], ref[:n], mag[:n], dtype, list(cache.lengths) + [1], np.abs(cache.v_ref).max())
+    if lse is not None:
+        got, l_ref = _np(lse)[:n], l_ref[:n]
+        none = np.isinf(l_ref)
+        assert (got[none] == -np.inf).all()
+        assert (np.abs(got[~none] - l_ref[~none])
+                <= 2.0 ** -13 + 2.0 ** -20 * np.abs(l_ref[~none])).all()
+
+
+# ------------------------------------------------------------------- append
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,page,hq,kv,half,inter,norm,layout", [
+    (128, 16, 4, 2, 64, False, True, "hnd"), (128, 64, 3, 3, 64, True, False, "nhd"),
+    (64, 32, 7, 1, 32, False, True, "nhd"), (64, 16, 1, 1, 8, True, True, "hnd"),
+    (128, 128, 5, 5, 16, False, False, "hnd"), (64, 256, 16, 2, 24, False, True, "hnd"),
+    (128, 16, 2, 1, 0, False, True, "hnd"), (64, 16, 2, 2, 0, False, False, "hnd")])
+def test_append(cuda, dtype, dim, page, hq, kv, half, inter, norm, layout):
+    from hybrid_llm_b200 import kernels
+    dt = DT[dtype]
+    new = [5, 0, 1, 40, 17, 3]
+    lengths = [5, 9, 300, 41, 17, 0]  # the last has tokens but no positions
+    cache = Cache(lengths, kv, dim, page, dt, seed=dim + page + hq, layout=layout)
+    rng = np.random.default_rng(5)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    n = cu[-1] + 4                    # rows behind the last sequence
+    fused = torch.from_numpy(rng.normal(size=(n, (hq + 2 * kv) * dim)).astype(np.float32)).to(dt)
+    fused = fused.cuda()
+    q = fused[:, :hq * dim].view(n, hq, dim)
+    k = fused[:, hq * dim:(hq + kv) * dim].view(n, kv, dim)
+    v = fused[:, (hq + kv) * dim:].view(n, kv, dim)
+    inv = torch.tensor(10000.0 ** (-np.arange(half) / max(half, 1)), dtype=torch.float32).cuda()
+    wq, wk = (torch.from_numpy(rng.normal(1, 0.3, dim).astype(np.float32)).cuda() if norm else None
+              for _ in range(2))
+    q_out = torch.full((n, hq, dim), 7.0, dtype=dt, device="cuda")
+    before = cache.kd.clone(), cache.vd.clone()
+    got = kernels.paged_append(q, k, v, cache.kd, cache.vd, cache.td, cache.ld,
+                               cu_q=torch.from_numpy(cu.astype(np.int32)).cuda(),
+                               inv_freq=inv if half else None, interleaved=inter, q_norm=wq,
+                               k_norm=wk, q_out=q_out)
+    kernels.check_device_status()
+    assert got is q_out
+    seq, pos = paged.positions(cu, lengths, n)
+    live = (seq >= 0) & (pos >= 0)
+    args = (1e-6, pos, inv.cpu().numpy() if half else None, inter)
+    assert (q_out[cu[-1]:] == 7.0).all()
+    assert (q_out[torch.from_numpy((seq >= 0) & (pos < 0)).cuda()] == 0).all()
+    stored = np.zeros((cache.pages, page), bool)
+    for name, x, w, heads in (("q", q, wq, hq), ("k", k, wk, kv)):
+        w = None if w is None else w.cpu().numpy()
+        ref = paged.norm_rotate(_np(x), w, *args)
+        plain = paged.norm_rotate(_np(x), w, 1e-6, pos, None, inter)
+        size = np.abs(plain).max(-1, keepdims=True) * 2
+        tol = U[dt] * np.abs(ref) + 2e-6 * size
+        if name == "q":
+            have = _np(q_out)
+        else:
+            have = np.zeros_like(ref)
+            for i in np.flatnonzero(live):
+                p, r = cache.table[seq[i], pos[i] // page], pos[i] % page
+                stored[p, r] = True
+                have[i] = _np(cache.kd[p, :, r])
+                assert torch.equal(cache.vd[p, :, r], v[i])
+        assert (np.abs(have - ref)[live] <= tol[live]).all(), name
+    keep = torch.from_numpy(~stored).cuda()[:, None, :, None].expand(cache.k.shape)
+    for was, now in zip(before, (cache.kd, cache.vd)):
+        assert torch.equal(was[keep].view(torch.int16), now[keep].view(torch.int16))
+
+
+def test_append_far_positions_and_in_place(cuda):
+    """Angles at a position near 10^6; q_out is q; one token per sequence."""
+    from hybrid_llm_b200 import kernels
+    page, far = 256, 999_937
+    width = far // page + 1
+    table = torch.zeros(2, width, dtype=torch.int32, device="cuda")
+    table[0, far // page], table[1, 0] = 1, 0
+    kp, vp = (torch.zeros(2, 2, page, 128, dtype=torch.float16, device="cuda") for _ in range(2))
+    lengths = torch.tensor([far + 1, 3], dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn(2, 4, 128, generator=g, device="cuda").half()
+    k = torch.randn(2, 2, 128, generator=g, device="cuda").half()
+    inv = (10000.0 ** (-torch.arange(64, device="cuda", dtype=torch.float64) / 64)).float()
+    ref = paged.norm_rotate(_np(q), None, 0, [far, 2], inv.cpu().numpy(), False)
+    tol = U[torch.float16] * np.abs(ref) + 4e-6 * np.abs(_np(q)).max()
+    out = kernels.paged_append(q, k, k, kp, vp, table, lengths, inv_freq=inv, q_out=q)
+    kernels.check_device_status()
+    assert out is q and (np.abs(_np(q) - ref) <= tol).all()
+    assert torch.equal(vp[1, :, far % page], k[0])
+
+
+def test_append_bad_page_is_reported_and_skipped(cuda):
+    from hybrid_llm_b200 import kernels
+    kp = torch.zeros(2, 1, 16, 64, dtype=torch.bfloat16, device="cuda")
+    vp = torch.zeros_like(kp)
+    x = torch.ones(3, 1, 64, dtype=torch.bfloat16, device="cuda")
+    table = torch.tensor([[0], [-1], [2]], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([1, 1, 1], dtype=torch.int32, device="cuda")
+    kernels.paged_append(x, x, x, kp, vp, table, lengths)
+    with pytest.raises(RuntimeError, match="invalid argument"):
+        kernels.check_device_status()
+    kernels.check_device_status()  # reported once
+    assert float(vp.sum()) == 64.0
+
+
+# ------------------------------------------------------------------- decode
+DECODE = [
+    # lengths, hq, kv, dim, page, softcap, window, alibi, layout
+    ([1], 1, 1, 128, 16, 0, 0, False, "hnd"),
+    ([0], 4, 2, 64, 16, 0, 0, False, "hnd"),
+    ([0, 1, 0, 15, 16, 17, 0], 4, 2, 128, 16, 0, 0, False, "hnd"),
+    ([31, 32, 33, 1000], 6, 2, 64, 16, 0, 0, False, "nhd"),
+    ([777], 8, 1, 128, 64, 30.0, 0, False, "hnd"),
+    ([513, 64, 63, 65], 5, 5, 64, 32, 0, 0, True, "hnd"),
+    ([300, 5, 999], 7, 1, 128, 128, 20.0, 100, True, "nhd"),
+    ([256, 257, 1], 20, 1, 64, 256, 0, 1, False, "hnd"),
+    ([400] * 40, 16, 8, 64, 16, 0, 37, False, "hnd"),
+    ([5000, 3], 33, 1, 128, 16, 0, 0, False, "hnd"),
+    (list(range(0, 330, 3)), 4, 4, 128, 32, 50.0, 0, False, "hnd"),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("lengths,hq,kv,dim,page,softcap,window,alibi,layout", DECODE)
+def test_decode(cuda, dtype, lengths, hq, kv, dim, page, softcap, window, alibi, layout):
+    from hybrid_llm_b200 import kernels
+    dt = DT[dtype]
+    cache = Cache(lengths, kv, dim, page, dt, seed=len(lengths) + hq, layout=layout)
+    g = torch.Generator().manual_seed(2)
+    b = len(lengths)
+    wide = torch.randn(b, hq + 1, dim + 8, generator=g).to(dt).cuda()
+    q = wide[:, 1:, 8:]  # strided rows and heads
+    slopes = torch.rand(hq, generator=g).cuda() if alibi else None
+    out = torch.full((b, hq, dim), 9.0, dtype=dt, device="cuda")
+    lse = torch.full((b, hq), 9.0, device="cuda")
+    kernels.paged_decode(q, cache.kd, cache.vd, cache.td, cache.ld, softcap=softcap,
+                         window=window, slopes=slopes, out=out, lse=lse)
+    kernels.check_device_status()
+    _check(out, lse, cache, q, np.arange(b + 1), dt, softcap=softcap, window=window,
+           slopes=None if slopes is None else _np(slopes))
+
+
+def test_decode_window_pages_may_be_gone(cuda):
+    """Pages wholly before the window are not looked at: their entries may be anything."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([500, 90], 2, 64, 16, torch.bfloat16, seed=3)
+    q = torch.randn(2, 4, 64, device="cuda").bfloat16()
+    table = cache.td.clone()
+    table[0, :(500 - 50) // 16] = -7
+    table[1, :(90 - 50) // 16] = 1 << 30
+    out = kernels.paged_decode(q, cache.kd, cache.vd, table, cache.ld, window=50)
+    kernels.check_device_status()
+    _check(out, None, cache, q, np.arange(3), torch.bfloat16, window=50)
+
+
+def test_bad_pages_and_lengths_are_reported(cuda):
+    """A page number out of range, and a length that the table cannot hold, reach no memory."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([40, 20], 1, 64, 16, torch.bfloat16, seed=4, pad=0)
+    q = torch.randn(2, 1, 64, device="cuda").bfloat16()
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    for entry in (cache.pages, -1, 1 << 30):
+        table = cache.td.clone()
+        table[0, 1] = entry
+        for call in (lambda: kernels.paged_decode(q, cache.kd, cache.vd, table, cache.ld),
+                     lambda: kernels.paged_prefill(q, cache.kd, cache.vd, table, cache.ld, cu)):
+            call()
+            with pytest.raises(RuntimeError, match="invalid argument"):
+                kernels.check_device_status()
+
+
+def test_decode_long_context_many_splits(cuda):
+    """One sequence over every worker, scores far apart (the maximum moves late)."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([20011], 2, 128, 64, torch.bfloat16, seed=6)
+    g = torch.Generator().manual_seed(8)
+    q = (torch.randn(1, 6, 128, generator=g) * 6).bfloat16().cuda()
+    lse = torch.empty(1, 6, device="cuda")
+    out = kernels.paged_decode(q, cache.kd, cache.vd, cache.td, cache.ld, lse=lse)
+    kernels.check_device_status()
+    ref, mag, _ = paged.attention(_np(q), cache.k_ref, cache.v_ref, cache.table, cache.lengths,
+                                  [0, 1], scale=128 ** -0.5)
+    # six times the scores: 6 2^-13 of their rounding
+    tol = U[torch.bfloat16] * np.abs(ref) + (U[torch.bfloat16] + 6 * 2.0 ** -12) * mag
+    assert (np.abs(_np(out) - ref) <= tol).all()
+    again = kernels.paged_decode(q, cache.kd, cache.vd, cache.td, cache.ld)
+    assert torch.equal(out, again)
+
+
+# ------------------------------------------------------------------ prefill
+PREFILL = [
+    # new, context, hq, kv, dim, page, softcap, window, alibi, prefix, layout
+    ([1], [0], 1, 1, 128, 16, 0, 0, False, None, "hnd"),
+    ([7], [0], 4, 2, 64, 16, 0, 0, False, None, "hnd"),
+    ([130, 1, 0, 257], [0, 300, 50, 3], 4, 4, 128, 32, 0, 0, False, None, "hnd"),
+    ([128, 256, 64], [0, 0, 64], 2, 1, 64, 64, 0, 0, False, None, "nhd"),
+    ([600], [0], 3, 1, 128, 128, 30.0, 0, False, None, "hnd"),
+    ([90, 333], [1000, 17], 5, 1, 64, 16, 0, 0, True, None, "hnd"),
+    ([300, 40], [200, 700], 8, 2, 128, 16, 20.0, 100, True, None, "nhd"),
+    ([257, 100], [0, 500], 4, 4, 64, 256, 0, 1, False, None, "hnd"),
+    ([200, 300, 50], [0, 100, 400], 4, 1, 128, 64, 0, 0, False, [150, 0, 9999], "hnd"),
+    ([150, 65], [20, 0], 6, 3, 64, 32, 10.0, 0, True, [165, 64], "nhd"),
+    ([5, 3], [2000, 3000], 16, 1, 128, 16, 0, 0, False, None, "hnd"),
+    ([33], [100], 33, 1, 64, 16, 0, 50, False, None, "hnd"),
+    ([3], [40], 128, 1, 64, 16, 0, 0, False, None, "hnd"),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("new,context,hq,kv,dim,page,softcap,window,alibi,prefix,layout", PREFILL)
+def test_prefill(cuda, dtype, new, context, hq, kv, dim, page, softcap, window, alibi, prefix,
+                 layout):
+    from hybrid_llm_b200 import kernels
+    dt = DT[dtype]
+    lengths = [a + b for a, b in zip(new, context)]
+    cache = Cache(lengths, kv, dim, page, dt, seed=sum(new) + hq, layout=layout)
+    g = torch.Generator().manual_seed(3)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    n = cu[-1] + 3  # rows behind the last sequence
+    wide = torch.randn(n, hq + 1, dim + 8, generator=g).to(dt)
+    wide[cu[-1]:] = float("nan")
+    q = wide.cuda()[:, 1:, 8:]
+    slopes = torch.rand(hq, generator=g).cuda() if alibi else None
+    pre = None if prefix is None else torch.tensor(prefix, dtype=torch.int32, device="cuda")
+    out = torch.full((n, hq, dim), 9.0, dtype=dt, device="cuda")
+    lse = torch.full((n, hq), 9.0, device="cuda")
+    kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld,
+                          torch.from_numpy(cu.astype(np.int32)).cuda(), softcap=softcap,
+                          window=window, slopes=slopes, prefix=pre, out=out, lse=lse)
+    kernels.check_device_status()
+    assert (out[cu[-1]:] == 9.0).all() and (lse[cu[-1]:] == 9.0).all()
+    _check(out, lse, cache, q[:cu[-1]], cu, dt, softcap=softcap, window=window,
+           slopes=None if slopes is None else _np(slopes), prefix=prefix)
+
+
+def test_prefill_rows_without_keys(cuda):
+    """Tokens before position 0 (a length shorter than the tokens) see nothing: zeros."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([4, 0, 130], 1, 64, 16, torch.bfloat16, seed=9)
+    new = [10, 5, 140]
+    cu = np.concatenate([[0], np.cumsum(new)])
+    q = torch.randn(cu[-1], 2, 64, device="cuda").bfloat16()
+    pre = torch.tensor([3, 2, 100], dtype=torch.int32, device="cuda")
+    lse = torch.empty(cu[-1], 2, device="cuda")
+    for p in (None, pre):
+        out = kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld,
+                                    torch.from_numpy(cu.astype(np.int32)).cuda(), prefix=p, lse=lse)
+        kernels.check_device_status()
+        _check(out, lse, cache, q, cu, torch.bfloat16, prefix=None if p is None else [3, 2, 100])
+        assert (out[:6] == 0).all() and (lse[:6] == -float("inf")).all()
+
+
+def test_prefill_many_units_and_moving_maximum(cuda):
+    """More units than SMs, ragged, with a few large scores; repeated bit for bit."""
+    from hybrid_llm_b200 import kernels
+    new = [900, 1, 513, 256, 700, 31, 640, 333]
+    context = [0, 250, 128, 77, 0, 0, 1, 500]
+    lengths = [a + b for a, b in zip(new, context)]
+    cache = Cache(lengths, 8, 64, 32, torch.bfloat16, seed=12)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(cu[-1], 16, 64, generator=g)
+    q[::97] *= 6
+    q = q.bfloat16().cuda()
+    cud = torch.from_numpy(cu.astype(np.int32)).cuda()
+    out = kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld, cud)
+    kernels.check_device_status()
+    ref, mag, _ = paged.attention(_np(q), cache.k_ref, cache.v_ref, cache.table, lengths, cu,
+                                  scale=0.125)
+    tol = U[torch.bfloat16] * np.abs(ref) + (U[torch.bfloat16] + 6 * 2.0 ** -12) * mag
+    assert (np.abs(_np(out) - ref) <= tol).all()
+    for _ in range(4):
+        assert torch.equal(out, kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld, cud))
+
+
+def test_prefill_one_token_equals_decode(cuda):
+    """One new token per sequence through both operators, within both roundings."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([77, 1, 300], 2, 128, 16, torch.bfloat16, seed=13)
+    q = torch.randn(3, 8, 128, device="cuda").bfloat16()
+    cu = torch.arange(4, dtype=torch.int32, device="cuda")
+    a = kernels.paged_decode(q, cache.kd, cache.vd, cache.td, cache.ld)
+    b = kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld, cu)
+    kernels.check_device_status()
+    for x in (a, b):
+        _check(x, None, cache, q, np.arange(4), torch.bfloat16)
+
+
+# ----------------------------------------------------------------- together
+def test_conversation(cuda):
+    """A prompt in two chunks, then tokens one by one: append, attend, per step."""
+    from hybrid_llm_b200 import kernels
+    rng = np.random.default_rng(20)
+    hq, kv, dim, page, b = 4, 2, 64, 16, 3
+    chunks = [[40, 7, 100], [21, 30, 0]] + [[1, 1, 1]] * 5
+    total = np.sum(chunks, 0)
+    cache = Cache(list(total), kv, dim, page, torch.bfloat16, seed=21)
+    inv = torch.tensor(10000.0 ** (-np.arange(32) / 32), dtype=torch.float32).cuda()
+    wq, wk = (torch.from_numpy(rng.normal(1, 0.2, dim).astype(np.float32)).cuda() for _ in range(2))
+    done = np.zeros(b, np.int64)
+    k_ref, v_ref = np.zeros_like(cache.k_ref), np.zeros_like(cache.v_ref)
+    for new in chunks:
+        done = done + new
+        cu = np.concatenate([[0], np.cumsum(new)])
+        n = cu[-1]
+        ld = torch.from_numpy(done.astype(np.int32)).cuda()
+        cud = torch.from_numpy(cu.astype(np.int32)).cuda()
+        x = torch.from_numpy(rng.normal(size=(n, hq + 2 * kv, dim)).astype(np.float32)).bfloat16().cuda()
+        q, k, v = x[:, :hq], x[:, hq:hq + kv], x[:, hq + kv:]
+        single = max(new) == 1
+        qr = kernels.paged_append(q, k, v, cache.kd, cache.vd, cache.td, ld,
+                                  cu_q=None if single else cud, inv_freq=inv, q_norm=wq, k_norm=wk)
+        out = (kernels.paged_decode(qr, cache.kd, cache.vd, cache.td, ld) if single else
+               kernels.paged_prefill(qr, cache.kd, cache.vd, cache.td, ld, cud))
+        kernels.check_device_status()
+        # the oracle attends over the rows that the append stored
+        seq, pos = paged.positions(cu, done, n)
+        kk = paged.norm_rotate(_np(k), wk.cpu().numpy(), 1e-6, pos, inv.cpu().numpy(), False)
+        for i in range(n):
+            p, r = cache.table[seq[i], pos[i] // page], pos[i] % page
+            have = _np(cache.kd[p, :, r])
+            assert np.abs(have - kk[i]).max() <= 2.0 ** -8 * np.abs(kk[i]).max() + 1e-5
+            k_ref[p, :, r], v_ref[p, :, r] = have, _np(v[i])
+        cache.k_ref, cache.v_ref, cache.lengths = k_ref, v_ref, done
+        _check(out, None, cache, qr, cu, torch.bfloat16)
+
+
+def test_captured_step_follows_its_inputs(cuda):
+    """A captured append + decode step replayed with growing lengths, on another
+    stream than its inputs', with a second graph of the same kind between."""
+    from hybrid_llm_b200 import kernels
+    page, dim, hq, kv = 16, 128, 4, 2
+    lengths = [200, 31]
+    caches = [Cache(lengths, kv, dim, page, torch.bfloat16, seed=s) for s in (30, 31)]
+    stream = torch.cuda.Stream()
+    graphs = []
+    for c in caches:
+        c.x = torch.zeros(2, hq + 2 * kv, dim, dtype=torch.bfloat16, device="cuda")
+        c.n = torch.tensor([1, 1], dtype=torch.int32, device="cuda")
+
+        def step(c=c):
+            q = kernels.paged_append(c.x[:, :hq], c.x[:, hq:hq + kv], c.x[:, hq + kv:], c.kd, c.vd,
+                                     c.td, c.n)
+            return kernels.paged_decode(q, c.kd, c.vd, c.td, c.n)
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            step()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                c.out = step()
+        graphs.append(g)
+        first = c.table[:, 0]  # the uncaptured step stored zero rows at position 0
+        c.k_ref[first, :, 0], c.v_ref[first, :, 0] = 0.0, 0.0
+    g = torch.Generator().manual_seed(5)
+    for length in ([150, 9], [151, 10], [200, 31]):
+        for c, graph in zip(caches, graphs):
+            c.x.copy_(torch.randn(c.x.shape, generator=g).bfloat16())
+            c.n.copy_(torch.tensor(length, dtype=torch.int32))
+            graph.replay()
+        torch.cuda.synchronize()
+        kernels.check_device_status()
+        for c in caches:
+            for b in range(2):
+                p, r = c.table[b, (length[b] - 1) // page], (length[b] - 1) % page
+                c.k_ref[p, :, r], c.v_ref[p, :, r] = _np(c.x[b, hq:hq + kv]), _np(c.x[b, hq + kv:])
+            c.lengths = np.asarray(length)
+            _check(c.out, None, c, c.x[:, :hq], np.arange(3), torch.bfloat16)
+
+
+def test_two_streams_at_once(cuda):
+    """Two decodes and two prefills in flight on two streams, each with its own scratch."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([3000, 40], 2, 64, 16, torch.bfloat16, seed=40)
+    q = torch.randn(2, 4, 64, device="cuda").bfloat16()
+    cu = torch.arange(3, dtype=torch.int32, device="cuda")
+    want = kernels.paged_decode(q, cache.kd, cache.vd, cache.td, cache.ld)
+    want_p = kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld, cu)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append((kernels.paged_decode(q, cache.kd, cache.vd, cache.td, cache.ld),
+                            kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld, cu)))
+    torch.cuda.synchronize()
+    kernels.check_device_status()
+    for d, p in got:
+        assert torch.equal(d, want) and torch.equal(p, want_p)
+
+
+def test_refusals(cuda):
+    from hybrid_llm_b200 import kernels
+    cache = Cache([40], 2, 64, 16, torch.bfloat16, seed=50)
+    q = torch.randn(1, 4, 64, device="cuda").bfloat16()
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    ok = (cache.kd, cache.vd, cache.td, cache.ld)
+    kv = q[:, :2]
+
+    def refused(f, *a, **kw):
+        with pytest.raises(ValueError):
+            f(*a, **kw)
+    for f, tail in ((kernels.paged_decode, ()), (kernels.paged_prefill, (cu,))):
+        refused(f, q.half(), *ok, *tail)
+        refused(f, q[:, :3], *ok, *tail)                       # 3 heads over 2
+        refused(f, q[..., :32], *ok, *tail)
+        refused(f, q, cache.kd[..., :32], cache.vd[..., :32], cache.td, cache.ld, *tail)
+        refused(f, q, cache.kd, cache.vd.transpose(1, 2).contiguous().transpose(1, 2), cache.td,
+                cache.ld, *tail)
+        refused(f, q, cache.kd[:, :, :8], cache.vd[:, :, :8], cache.td, cache.ld, *tail)
+        refused(f, q, cache.kd, cache.vd, cache.td.long(), cache.ld, *tail)
+        refused(f, q, cache.kd, cache.vd, cache.td, cache.ld.long(), *tail)
+        refused(f, q, *ok, *tail, scale=0.0)
+        refused(f, q, *ok, *tail, scale=float("nan"))
+        refused(f, q, *ok, *tail, softcap=-1.0)
+        refused(f, q, *ok, *tail, window=-1)
+        refused(f, q, *ok, *tail, slopes=torch.ones(3, device="cuda"))
+        refused(f, q, *ok, *tail, out=torch.empty(1, 4, 64, device="cuda"))
+        refused(f, q, *ok, *tail, lse=torch.empty(4, device="cuda"))
+        with pytest.raises(RuntimeError):
+            f(q.cpu(), *ok, *tail)
+    refused(kernels.paged_decode, torch.cat([q, q]), *ok)
+    refused(kernels.paged_prefill, q, *ok, cu.long())
+    refused(kernels.paged_prefill, q, *ok, cu, window=4, prefix=cache.ld)
+    refused(kernels.paged_append, q, kv, kv[:, :1], *ok)
+    refused(kernels.paged_append, torch.cat([q, q]), torch.cat([kv, kv]), torch.cat([kv, kv]), *ok)
+    refused(kernels.paged_append, q, kv, kv, *ok, inv_freq=torch.ones(12, device="cuda"))
+    refused(kernels.paged_append, q, kv, kv, *ok, inv_freq=torch.ones(40, device="cuda"))
+    refused(kernels.paged_append, q, kv, kv, *ok, q_norm=torch.ones(32, device="cuda"))
+
+
+def test_empty_calls(cuda):
+    """No sequences, or sequences without tokens."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([40], 2, 64, 16, torch.bfloat16, seed=50)
+    q = torch.empty(0, 4, 64, dtype=torch.bfloat16, device="cuda")
+    none = torch.zeros(1, dtype=torch.int32, device="cuda")
+    t, l = cache.td[:0], cache.ld[:0]
+    assert kernels.paged_decode(q, cache.kd, cache.vd, t, l).shape == q.shape
+    assert kernels.paged_prefill(q, cache.kd, cache.vd, t, l, none).shape == q.shape
+    assert kernels.paged_append(q, q[:, :2], q[:, :2], cache.kd, cache.vd, t, l,
+                                cu_q=none).shape == q.shape
+    two = torch.zeros(2, dtype=torch.int32, device="cuda")
+    assert kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld, two).shape == q.shape
+    row = torch.full((1, 4, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    out = row.clone()
+    kernels.paged_prefill(row, cache.kd, cache.vd, cache.td, cache.ld, two, out=out)
+    assert torch.equal(out, row)
+    kernels.check_device_status()

@@ -7,6 +7,7 @@ call raises, so a GPU run can never silently take a CPU or eager path.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 import threading
 from pathlib import Path
 
@@ -127,17 +128,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "llmyb_router_ctx_prefill": (I32, [P, I32, I32, I32, I32, P, P, P, P, P]),
     "llmyb_router_ctx_step": (I32, [P, I32, I32, I32, P, P, P, P, P, P]),
     # paged key-value cache
-    "llmyb_paged_append": (I32, [P, I64, I64, P, I64, I64, P, I64, I64, I32, I32, I32, I32, I32, P,
-                                 P, I64, I64, I64, I32, I32, P, I64, I32, P, P, I32, P, P, F32, P,
-                                 I32, I32, P, I64, I64, P, P]),
+    "llmyb_paged_append": (I32, [C.c_char_p, P]),
     "llmyb_paged_decode_scratch_bytes": (I64, [I32, I32, I32]),
-    "llmyb_paged_decode": (I32, [P, I64, I64, I32, I32, I32, I32, I32, P, P, I64, I64, I64, I32,
-                                 I32, P, I64, I32, P, F32, F32, I32, P, P, I64, I64, P, P, P, P]),
+    "llmyb_paged_decode": (I32, [C.c_char_p, P]),
     "llmyb_paged_prefill_scratch_bytes": (I64, [I32, I32, I32, I32, I32, I32]),
-    "llmyb_paged_prefill": (I32, [P, I64, I64, I32, I32, I32, I32, I32, P, P, I64, I64, I64, I32,
-                                  I32, P, I64, I32, P, P, I32, P, F32, F32, I32, P, P, I64, I64, P,
-                                  P, P, P]),
+    "llmyb_paged_prefill": (I32, [C.c_char_p, P]),
 }
+
+# llmyb_paged_args of include/llmyb.h: 17 pointers, 12 strides, 12 int32, 3
+# floats, 1 int32.  A packed block costs a tenth of ctypes' conversion of as
+# many arguments, which would be most of a one-token call.
+PAGED_ARGS = struct.Struct("=17Q12q12i3fi")
 
 _lock = threading.Lock()
 _lib: C.CDLL | None = None

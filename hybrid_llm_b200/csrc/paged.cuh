@@ -10,6 +10,7 @@
 
 #include <cuda_fp16.h>
 #include "common.cuh"
+#include "../../include/llmyb.h"
 
 namespace llmyb {
 
@@ -95,6 +96,44 @@ inline int page_shift_of(int page_size) {
     case 256: return 8;
     default: return -1;
   }
+}
+
+inline bool paged_aligned(const void* p, int64_t a = 0, int64_t b = 0) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && a % 8 == 0 && b % 8 == 0;
+}
+
+// What the three calls check alike: LLMYB_OK, or why not.  Call it before
+// anything else; a call without tokens or sequences needs no pointers.
+inline int32_t paged_check(const llmyb_paged_args* a) {
+  if (!a || a->n_tokens < 0 || a->batch < 0 || a->q_heads <= 0 || a->kv_heads <= 0 ||
+      a->num_pages < 0 || a->table_width < 0)
+    return LLMYB_EINVAL;
+  if (a->n_tokens == 0 || a->batch == 0) return LLMYB_OK;
+  if (!a->q || !a->k_pages || !a->v_pages || !a->table || !a->lengths || !a->out ||
+      a->num_pages == 0)
+    return LLMYB_EINVAL;
+  const int shift = page_shift_of(a->page_size);
+  if (shift < 0 || (a->head_dim != 64 && a->head_dim != 128) ||
+      a->table_width > (1 << 30) >> shift ||
+      !paged_aligned(a->q, a->q_token_stride, a->q_head_stride) ||
+      !paged_aligned(a->out, a->out_token_stride, a->out_head_stride) ||
+      !paged_aligned(a->k_pages, a->page_stride, a->head_stride) ||
+      !paged_aligned(a->v_pages, a->row_stride))
+    return LLMYB_EUNSUPPORTED;
+  return LLMYB_OK;
+}
+
+// Further for the attention calls.
+inline int32_t paged_check_scores(const llmyb_paged_args* a) {
+  if (a->q_heads % a->kv_heads != 0 || a->window < 0 || !(a->scale > 0.f) || !(a->softcap >= 0.f))
+    return LLMYB_EINVAL;
+  return LLMYB_OK;
+}
+
+inline PagedPool paged_pool(const llmyb_paged_args* a) {
+  return {a->page_stride, a->head_stride, a->row_stride, a->num_pages,
+          page_shift_of(a->page_size), a->table, a->table_stride, a->table_width, a->lengths,
+          a->batch, a->kv_heads};
 }
 
 }  // namespace llmyb

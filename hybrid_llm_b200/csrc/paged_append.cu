@@ -162,62 +162,45 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a) {
   }
 }
 
-bool aligned(const void* p, int64_t a, int64_t b) {
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && a % 8 == 0 && b % 8 == 0;
-}
-
 }  // namespace
 }  // namespace llmyb
 
 using namespace llmyb;
 
-LLMYB_API int32_t llmyb_paged_append(
-    const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
-    int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
-    int64_t v_head_stride, int32_t n_tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
-    int32_t fp16, void* k_pages, void* v_pages, int64_t page_stride, int64_t head_stride,
-    int64_t row_stride, int32_t num_pages, int32_t page_size, const int32_t* table,
-    int64_t table_stride, int32_t table_width, const int32_t* lengths, const int32_t* cu_q,
-    int32_t batch, const float* q_norm, const float* k_norm, float eps, const float* inv_freq,
-    int32_t rope_half, int32_t interleaved, void* q_out, int64_t out_token_stride,
-    int64_t out_head_stride, int32_t* dev_status, void* stream) {
-  if (n_tokens < 0 || batch < 0 || q_heads <= 0 || kv_heads <= 0 || num_pages < 0 ||
-      table_width < 0 || rope_half < 0 || !(eps >= 0.f))
+LLMYB_API int32_t llmyb_paged_append(const llmyb_paged_args* x, void* stream) {
+  const int32_t st = paged_check(x);
+  if (st) return st;
+  if (x->rope_half < 0 || !(x->eps >= 0.f)) return LLMYB_EINVAL;
+  if (x->n_tokens == 0 || x->batch == 0) return LLMYB_OK;
+  if (!x->k || !x->v || (x->rope_half > 0 && !x->inv_freq) || (!x->cu_q && x->n_tokens != x->batch))
     return LLMYB_EINVAL;
-  if (n_tokens == 0 || batch == 0) return LLMYB_OK;
-  if (!q || !k || !v || !k_pages || !v_pages || !table || !lengths || !q_out ||
-      (rope_half > 0 && !inv_freq) || (!cu_q && n_tokens != batch))
-    return LLMYB_EINVAL;
-  const int shift = page_shift_of(page_size);
-  if (shift < 0 || (head_dim != 64 && head_dim != 128) || rope_half % 8 != 0 ||
-      2 * rope_half > head_dim || table_width > (1 << 30) >> shift)
-    return LLMYB_EUNSUPPORTED;
-  if (!aligned(q, q_token_stride, q_head_stride) || !aligned(k, k_token_stride, k_head_stride) ||
-      !aligned(v, v_token_stride, v_head_stride) || !aligned(q_out, out_token_stride, out_head_stride) ||
-      !aligned(k_pages, page_stride, head_stride) || !aligned(v_pages, row_stride, 0) ||
-      !aligned(q_norm, 0, 0) || !aligned(k_norm, 0, 0))
+  if (x->rope_half % 8 != 0 || 2 * x->rope_half > x->head_dim ||
+      !paged_aligned(x->k, x->k_token_stride, x->k_head_stride) ||
+      !paged_aligned(x->v, x->v_token_stride, x->v_head_stride) || !paged_aligned(x->q_norm) ||
+      !paged_aligned(x->k_norm))
     return LLMYB_EUNSUPPORTED;
   AppendArgs a;
-  a.q = static_cast<const uint16_t*>(q), a.k = static_cast<const uint16_t*>(k);
-  a.v = static_cast<const uint16_t*>(v);
-  a.q_tok = q_token_stride, a.q_head = q_head_stride;
-  a.k_tok = k_token_stride, a.k_head = k_head_stride;
-  a.v_tok = v_token_stride, a.v_head = v_head_stride;
-  a.q_out = static_cast<uint16_t*>(q_out), a.o_tok = out_token_stride, a.o_head = out_head_stride;
-  a.k_pages = static_cast<uint16_t*>(k_pages), a.v_pages = static_cast<uint16_t*>(v_pages);
-  a.pool = {page_stride, head_stride, row_stride, num_pages, shift,  table,
-            table_stride, table_width, lengths,   batch,     kv_heads};
-  a.cu_q = cu_q, a.n_tokens = n_tokens, a.q_heads = q_heads;
-  a.q_norm = q_norm, a.k_norm = k_norm, a.eps = eps;
-  a.inv_freq = inv_freq, a.half = rope_half, a.interleaved = interleaved;
-  a.dev_status = dev_status;
+  a.q = static_cast<const uint16_t*>(x->q), a.k = static_cast<const uint16_t*>(x->k);
+  a.v = static_cast<const uint16_t*>(x->v);
+  a.q_tok = x->q_token_stride, a.q_head = x->q_head_stride;
+  a.k_tok = x->k_token_stride, a.k_head = x->k_head_stride;
+  a.v_tok = x->v_token_stride, a.v_head = x->v_head_stride;
+  a.q_out = static_cast<uint16_t*>(x->out);
+  a.o_tok = x->out_token_stride, a.o_head = x->out_head_stride;
+  a.k_pages = static_cast<uint16_t*>(x->k_pages), a.v_pages = static_cast<uint16_t*>(x->v_pages);
+  a.pool = paged_pool(x);
+  a.cu_q = x->cu_q, a.n_tokens = x->n_tokens, a.q_heads = x->q_heads;
+  a.q_norm = x->q_norm, a.k_norm = x->k_norm, a.eps = x->eps;
+  a.inv_freq = x->inv_freq, a.half = x->rope_half, a.interleaved = x->interleaved;
+  a.dev_status = x->dev_status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (fp16) {
-    if (head_dim == 64) paged_append_kernel<__half, 64><<<n_tokens, kThreads, 0, s>>>(a);
-    else paged_append_kernel<__half, 128><<<n_tokens, kThreads, 0, s>>>(a);
+  const int n = x->n_tokens;
+  if (x->fp16) {
+    if (x->head_dim == 64) paged_append_kernel<__half, 64><<<n, kThreads, 0, s>>>(a);
+    else paged_append_kernel<__half, 128><<<n, kThreads, 0, s>>>(a);
   } else {
-    if (head_dim == 64) paged_append_kernel<__nv_bfloat16, 64><<<n_tokens, kThreads, 0, s>>>(a);
-    else paged_append_kernel<__nv_bfloat16, 128><<<n_tokens, kThreads, 0, s>>>(a);
+    if (x->head_dim == 64) paged_append_kernel<__nv_bfloat16, 64><<<n, kThreads, 0, s>>>(a);
+    else paged_append_kernel<__nv_bfloat16, 128><<<n, kThreads, 0, s>>>(a);
   }
   count_launch();
   return launch_status();

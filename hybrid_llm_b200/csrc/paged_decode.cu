@@ -472,10 +472,6 @@ int32_t launch(const DecodeArgs& a, cudaStream_t s) {
   return e == cudaSuccess ? launch_status() : static_cast<int32_t>(e);
 }
 
-bool aligned(const void* p, int64_t a, int64_t b) {
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && a % 8 == 0 && b % 8 == 0;
-}
-
 }  // namespace
 }  // namespace llmyb
 
@@ -488,47 +484,35 @@ LLMYB_API int64_t llmyb_paged_decode_scratch_bytes(int32_t q_heads, int32_t kv_h
   return static_cast<int64_t>(worker_count()) * 2 * rows * (head_dim + 2) * 4;
 }
 
-LLMYB_API int32_t llmyb_paged_decode(
-    const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t batch, int32_t q_heads,
-    int32_t kv_heads, int32_t head_dim, int32_t fp16, const void* k_pages, const void* v_pages,
-    int64_t page_stride, int64_t head_stride, int64_t row_stride, int32_t num_pages,
-    int32_t page_size, const int32_t* table, int64_t table_stride, int32_t table_width,
-    const int32_t* lengths, float scale, float softcap, int32_t window, const float* slopes,
-    void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, void* scratch,
-    int32_t* dev_status, void* stream) {
-  if (batch < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || num_pages < 0 ||
-      table_width < 0 || window < 0 || !(scale > 0.f) || !(softcap >= 0.f))
-    return LLMYB_EINVAL;
-  if (batch == 0) return LLMYB_OK;
-  if (!q || !k_pages || !v_pages || !table || !lengths || !out || !scratch) return LLMYB_EINVAL;
-  const int shift = page_shift_of(page_size);
-  if (shift < 0 || (head_dim != 64 && head_dim != 128) || table_width > (1 << 30) >> shift)
-    return LLMYB_EUNSUPPORTED;
-  if (!aligned(q, q_token_stride, q_head_stride) || !aligned(out, out_token_stride, out_head_stride) ||
-      !aligned(k_pages, page_stride, head_stride) || !aligned(v_pages, row_stride, 0) ||
-      !aligned(scratch, 0, 0))
-    return LLMYB_EUNSUPPORTED;
+LLMYB_API int32_t llmyb_paged_decode(const llmyb_paged_args* x, void* stream) {
+  int32_t st = paged_check(x);
+  if (st) return st;
+  st = paged_check_scores(x);
+  if (st) return st;
+  if (x->n_tokens != x->batch) return LLMYB_EINVAL;
+  if (x->batch == 0) return LLMYB_OK;
+  if (!x->scratch) return LLMYB_EINVAL;
+  if (!paged_aligned(x->scratch)) return LLMYB_EUNSUPPORTED;
   DecodeArgs a;
-  a.q = static_cast<const uint16_t*>(q), a.q_tok = q_token_stride, a.q_head = q_head_stride;
-  a.k_pages = static_cast<const uint16_t*>(k_pages);
-  a.v_pages = static_cast<const uint16_t*>(v_pages);
-  a.pool = {page_stride, head_stride, row_stride, num_pages, shift,  table,
-            table_stride, table_width, lengths,   batch,     kv_heads};
-  a.group = q_heads / kv_heads;
+  a.q = static_cast<const uint16_t*>(x->q), a.q_tok = x->q_token_stride, a.q_head = x->q_head_stride;
+  a.k_pages = static_cast<const uint16_t*>(x->k_pages);
+  a.v_pages = static_cast<const uint16_t*>(x->v_pages);
+  a.pool = paged_pool(x);
+  a.group = x->q_heads / x->kv_heads;
   a.chunks = (a.group + 15) / 16;
   a.rows = std::min(16, a.group);
-  a.q_heads = q_heads, a.window = window, a.workers = worker_count();
-  a.scale = scale, a.softcap = softcap, a.slopes = slopes;
-  a.out = static_cast<uint16_t*>(out), a.o_tok = out_token_stride, a.o_head = out_head_stride;
-  a.lse = lse;
-  a.part_o = static_cast<float*>(scratch);
+  a.q_heads = x->q_heads, a.window = x->window, a.workers = worker_count();
+  a.scale = x->scale, a.softcap = x->softcap, a.slopes = x->slopes;
+  a.out = static_cast<uint16_t*>(x->out);
+  a.o_tok = x->out_token_stride, a.o_head = x->out_head_stride;
+  a.lse = x->lse;
+  a.part_o = static_cast<float*>(x->scratch);
   a.part_ml = reinterpret_cast<float2*>(a.part_o +
-                                        static_cast<int64_t>(a.workers) * 2 * a.rows * head_dim);
-  a.dev_status = dev_status;
-  if (static_cast<int64_t>(batch) * kv_heads * a.chunks * a.rows > 0x7fffffffll)
+                                        static_cast<int64_t>(a.workers) * 2 * a.rows * x->head_dim);
+  a.dev_status = x->dev_status;
+  if (static_cast<int64_t>(x->batch) * x->kv_heads * a.chunks * a.rows > 0x7fffffffll)
     return LLMYB_EUNSUPPORTED;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (fp16)
-    return head_dim == 64 ? launch<__half, 64>(a, s) : launch<__half, 128>(a, s);
-  return head_dim == 64 ? launch<__nv_bfloat16, 64>(a, s) : launch<__nv_bfloat16, 128>(a, s);
+  if (x->fp16) return x->head_dim == 64 ? launch<__half, 64>(a, s) : launch<__half, 128>(a, s);
+  return x->head_dim == 64 ? launch<__nv_bfloat16, 64>(a, s) : launch<__nv_bfloat16, 128>(a, s);
 }

@@ -610,26 +610,25 @@ int most_splits(int n_tokens, int kv_heads, int tile_tokens, int table_width, in
 }
 
 template <typename T, int D>
-int32_t launch(const void* q, int64_t q_tok, int64_t q_head, const void* k_pages,
-               const void* v_pages, int page_size, const PrefillArgs& a, cudaStream_t s) {
+int32_t launch(const llmyb_paged_args* x, const PrefillArgs& a, cudaStream_t s) {
   using L = Layout<D>;
   int32_t st = ensure_smem(paged_prefill_kernel<T, D>, L::kSmem);
   if (st) return st;
   CUtensorMap mq, mk, mv;
   {
     const uint64_t dims[3] = {D, static_cast<uint64_t>(a.q_heads), static_cast<uint64_t>(a.n_tokens)};
-    const int64_t strides[3] = {1, q_head, q_tok};
+    const int64_t strides[3] = {1, x->q_head_stride, x->q_token_stride};
     const uint32_t box[3] = {64, static_cast<uint32_t>(a.group), static_cast<uint32_t>(a.tile_tokens)};
-    if (!make_map(&mq, q, 3, dims, strides, box)) return LLMYB_EUNSUPPORTED;
+    if (!make_map(&mq, x->q, 3, dims, strides, box)) return LLMYB_EUNSUPPORTED;
   }
   {
-    const uint64_t dims[4] = {D, static_cast<uint64_t>(page_size),
+    const uint64_t dims[4] = {D, static_cast<uint64_t>(x->page_size),
                               static_cast<uint64_t>(a.pool.kv_heads),
                               static_cast<uint64_t>(a.pool.num_pages)};
     const int64_t strides[4] = {1, a.pool.row_stride, a.pool.head_stride, a.pool.page_stride};
-    const uint32_t box[4] = {64, static_cast<uint32_t>(std::min(page_size, kRows)), 1, 1};
-    if (!make_map(&mk, k_pages, 4, dims, strides, box) ||
-        !make_map(&mv, v_pages, 4, dims, strides, box))
+    const uint32_t box[4] = {64, static_cast<uint32_t>(std::min(x->page_size, kRows)), 1, 1};
+    if (!make_map(&mk, x->k_pages, 4, dims, strides, box) ||
+        !make_map(&mv, x->v_pages, 4, dims, strides, box))
       return LLMYB_EUNSUPPORTED;
   }
   const int grid = num_sms();
@@ -642,10 +641,6 @@ int32_t launch(const void* q, int64_t q_tok, int64_t q_head, const void* k_pages
                              dim3(kJoinThreads), 0, s, a, grid);
   count_launch();
   return e == cudaSuccess ? launch_status() : static_cast<int32_t>(e);
-}
-
-bool aligned(const void* p, int64_t a, int64_t b) {
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && a % 8 == 0 && b % 8 == 0;
 }
 
 }  // namespace
@@ -666,52 +661,32 @@ LLMYB_API int64_t llmyb_paged_prefill_scratch_bytes(int32_t n_tokens, int32_t q_
   return splits * n_tokens * q_heads * (head_dim + 2) * 4;
 }
 
-LLMYB_API int32_t llmyb_paged_prefill(
-    const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t n_tokens,
-    int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t fp16, const void* k_pages,
-    const void* v_pages, int64_t page_stride, int64_t head_stride, int64_t row_stride,
-    int32_t num_pages, int32_t page_size, const int32_t* table, int64_t table_stride,
-    int32_t table_width, const int32_t* lengths, const int32_t* cu_q, int32_t batch,
-    const int32_t* prefix, float scale, float softcap, int32_t window, const float* slopes,
-    void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, void* scratch,
-    int32_t* dev_status, void* stream) {
-  if (n_tokens < 0 || batch < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 ||
-      num_pages < 0 || table_width < 0 || window < 0 || !(scale > 0.f) || !(softcap >= 0.f) ||
-      (prefix && window > 0))
-    return LLMYB_EINVAL;
-  if (n_tokens == 0 || batch == 0) return LLMYB_OK;
-  if (!q || !k_pages || !v_pages || !table || !lengths || !cu_q || !out || num_pages == 0)
-    return LLMYB_EINVAL;
-  const int shift = page_shift_of(page_size);
-  const int group = q_heads / kv_heads;
-  if (shift < 0 || (head_dim != 64 && head_dim != 128) || group > kRows ||
-      table_width > (1 << 30) >> shift)
-    return LLMYB_EUNSUPPORTED;
-  if (!aligned(q, q_token_stride, q_head_stride) || !aligned(out, out_token_stride, out_head_stride) ||
-      !aligned(k_pages, page_stride, head_stride) || !aligned(v_pages, row_stride, 0) ||
-      !aligned(scratch, 0, 0))
-    return LLMYB_EUNSUPPORTED;
+LLMYB_API int32_t llmyb_paged_prefill(const llmyb_paged_args* x, void* stream) {
+  int32_t st = paged_check(x);
+  if (st) return st;
+  st = paged_check_scores(x);
+  if (st) return st;
+  if (x->prefix && x->window > 0) return LLMYB_EINVAL;
+  if (x->n_tokens == 0 || x->batch == 0) return LLMYB_OK;
+  if (!x->cu_q) return LLMYB_EINVAL;
+  const int group = x->q_heads / x->kv_heads;
+  if (group > kRows || !paged_aligned(x->scratch)) return LLMYB_EUNSUPPORTED;
   PrefillArgs a;
-  a.pool = {page_stride, head_stride, row_stride, num_pages, shift,  table,
-            table_stride, table_width, lengths,   batch,     kv_heads};
-  a.cu_q = cu_q, a.prefix = prefix, a.n_tokens = n_tokens, a.q_heads = q_heads, a.group = group;
-  a.tile_tokens = kRows / group;
-  a.window = window, a.scale = scale, a.softcap = softcap, a.slopes = slopes;
-  a.max_splits = most_splits(n_tokens, kv_heads, a.tile_tokens, table_width, page_size);
-  if (a.max_splits > 1 && !scratch) return LLMYB_EINVAL;
-  a.out = static_cast<uint16_t*>(out), a.o_tok = out_token_stride, a.o_head = out_head_stride;
-  a.lse = lse;
-  a.part_o = static_cast<float*>(scratch);
+  a.pool = paged_pool(x);
+  a.cu_q = x->cu_q, a.prefix = x->prefix, a.n_tokens = x->n_tokens, a.q_heads = x->q_heads;
+  a.group = group, a.tile_tokens = kRows / group;
+  a.window = x->window, a.scale = x->scale, a.softcap = x->softcap, a.slopes = x->slopes;
+  a.max_splits = most_splits(x->n_tokens, x->kv_heads, a.tile_tokens, x->table_width, x->page_size);
+  if (a.max_splits > 1 && !x->scratch) return LLMYB_EINVAL;
+  a.out = static_cast<uint16_t*>(x->out);
+  a.o_tok = x->out_token_stride, a.o_head = x->out_head_stride;
+  a.lse = x->lse;
+  a.part_o = static_cast<float*>(x->scratch);
   a.part_ml = reinterpret_cast<float2*>(
-      a.part_o + static_cast<int64_t>(a.max_splits) * n_tokens * q_heads * head_dim);
-  a.dev_status = dev_status;
+      a.part_o + static_cast<int64_t>(a.max_splits) * x->n_tokens * x->q_heads * x->head_dim);
+  a.dev_status = x->dev_status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (fp16)
-    return head_dim == 64
-               ? launch<__half, 64>(q, q_token_stride, q_head_stride, k_pages, v_pages, page_size, a, s)
-               : launch<__half, 128>(q, q_token_stride, q_head_stride, k_pages, v_pages, page_size, a, s);
-  return head_dim == 64 ? launch<__nv_bfloat16, 64>(q, q_token_stride, q_head_stride, k_pages,
-                                                    v_pages, page_size, a, s)
-                        : launch<__nv_bfloat16, 128>(q, q_token_stride, q_head_stride, k_pages,
-                                                     v_pages, page_size, a, s);
+  if (x->fp16) return x->head_dim == 64 ? launch<__half, 64>(x, a, s) : launch<__half, 128>(x, a, s);
+  return x->head_dim == 64 ? launch<__nv_bfloat16, 64>(x, a, s)
+                           : launch<__nv_bfloat16, 128>(x, a, s);
 }

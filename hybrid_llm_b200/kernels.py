@@ -1175,83 +1175,117 @@ def csa_remote_step(x: torch.Tensor, q: torch.Tensor, w_comp: torch.Tensor, rati
 
 
 # ------------------------------------------------------ paged key-value cache
+# These checks are most of a one-token call's host time: each attribute of a
+# tensor is asked for once.
 PAGE_SIZES = (16, 32, 64, 128, 256)
-_PAGED_DTYPES = (torch.bfloat16, torch.float16)
 
 
-def _paged_rows(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
-    """[N, heads, head_dim] rows of the cache's type."""
-    if t.dim() != 3 or t.dtype != like.dtype or t.shape[2] != like.shape[3]:
-        raise ValueError(f"{name} must be [tokens, heads, {like.shape[3]}] {like.dtype}")
-    sn, sh, sd = t.stride()
-    if sd != 1 or sn % 8 or sh % 8 or t.data_ptr() % 16:
+def _paged_rows(t: torch.Tensor, name: str, heads: int | None, dim: int, dtype: torch.dtype,
+                tokens: int | None = None):
+    """(pointer, token stride, head stride) of [tokens, heads, dim] rows."""
+    shape, (sn, sh, sd), p = t.shape, t.stride(), t.data_ptr()
+    if t.dtype is not dtype or shape[2] != dim or (heads is not None and shape[1] != heads) or (
+            tokens is not None and shape[0] != tokens):
+        raise ValueError(f"{name} must be [{tokens or 'tokens'}, {heads or 'heads'}, {dim}] {dtype}")
+    if sd != 1 or (sn | sh) & 7 or p & 15:
         raise ValueError(f"{name}: contiguous head dimension, 16-byte aligned rows and heads")
+    return p, sn, sh
 
 
-def _paged_i32(t: torch.Tensor, name: str, n: int) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.stride(0) != 1:
-        raise ValueError(f"{name} must be contiguous int32 [{n}]")
+def _paged_vector(t: torch.Tensor | None, name: str, dtype: torch.dtype, n: int) -> int:
+    if t is None:
+        return 0
+    if t.dtype is not dtype or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be contiguous {dtype} [{n}]")
+    return t.data_ptr()
 
 
-def _paged_f32(t: torch.Tensor | None, name: str, n: int | None = None) -> None:
-    if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or not t.is_contiguous()
-                          or (n is not None and t.shape[0] != n)):
-        raise ValueError(f"{name} must be contiguous fp32" + ("" if n is None else f" [{n}]"))
-
-
-def _paged_pool(k_pages, v_pages, block_table, lengths, *others):
-    """Checks the cache and the devices; returns the pool's ABI arguments."""
-    dev = torch.cuda.current_device() if k_pages.is_cuda else -1
-    for t in (k_pages, v_pages, block_table, lengths, *others):
-        if t is not None and t.get_device() != dev or dev < 0:
-            if t is not None and t.is_cuda and dev >= 0:
-                raise ValueError("paged cache tensors must be on the current CUDA device")
-            raise RuntimeError("llmyb kernels take CUDA tensors only (no CPU fallback)")
-    if (k_pages.dim() != 4 or k_pages.dtype not in _PAGED_DTYPES or k_pages.shape != v_pages.shape
-            or v_pages.dtype != k_pages.dtype or k_pages.stride() != v_pages.stride()):
+def _paged_call(entry: str, q, k_pages, v_pages, block_table, lengths, out, *, k=None, v=None,
+                cu_q=None, prefix=None, slopes=None, q_norm=None, k_norm=None, inv_freq=None,
+                lse=None, window=0, interleaved=False, scale=1.0, softcap=0.0, eps=0.0):
+    """Checks the arguments, allocates the output and the scratch, makes the call."""
+    dev = q.get_device()
+    for t in (k_pages, v_pages, block_table, lengths, out, k, v, cu_q, prefix, slopes, q_norm,
+              k_norm, inv_freq, lse):
+        if t is not None and t.get_device() != dev:
+            dev = -1
+    if dev < 0:
+        raise RuntimeError("llmyb kernels take CUDA tensors only (no CPU fallback), all on one "
+                           "device")
+    if dev != torch.cuda.current_device():
+        raise ValueError("paged cache tensors must be on the current CUDA device")
+    dtype, shape, strides = k_pages.dtype, k_pages.shape, k_pages.stride()
+    if (len(shape) != 4 or (dtype is not torch.bfloat16 and dtype is not torch.float16)
+            or v_pages.dtype is not dtype or v_pages.shape != shape
+            or v_pages.stride() != strides):
         raise ValueError("k_pages and v_pages must be alike: [pages, kv_heads, page_size, head_dim] "
                          "bf16 or fp16 with the same strides")
-    pages, _, page_size, dim = k_pages.shape
-    sp, sh, sr, sd = k_pages.stride()
-    if page_size not in PAGE_SIZES or dim not in (64, 128):
+    pages, kv_heads, page_size, dim = shape
+    sp, sh, sr, sd = strides
+    kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
+    if page_size not in PAGE_SIZES or (dim != 64 and dim != 128):
         raise ValueError(f"pages of {PAGE_SIZES} rows and head dimensions 64 or 128 are served")
-    if sd != 1 or sp % 8 or sh % 8 or sr % 8 or k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16:
+    if sd != 1 or (sp | sh | sr) & 7 or (kp | vp) & 15:
         raise ValueError("pages: contiguous head dimension, 16-byte aligned pages, heads and rows")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (
-            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    batch, width = block_table.shape
+    st, sc = block_table.stride()
+    if block_table.dtype is not torch.int32 or (sc != 1 and width > 1):
         raise ValueError("block_table must be int32 [batch, pages per sequence]")
-    _paged_i32(lengths, "lengths", block_table.shape[0])
-    return (sp, sh, sr, pages, page_size, block_table.data_ptr(), block_table.stride(0),
-            block_table.shape[1], lengths.data_ptr())
-
-
-def _paged_out(out, like: torch.Tensor, name: str = "out") -> torch.Tensor:
+    lp = _paged_vector(lengths, "lengths", torch.int32, batch)
+    if q.dim() != 3:
+        raise ValueError("q must be [tokens, heads, head_dim]")
+    n, heads, _ = q.shape
+    qp, qn, qh = _paged_rows(q, "q", None, dim, dtype)
+    kr = vr = (0, 0, 0)
+    half = 0
+    if k is not None:
+        kr = _paged_rows(k, "k", kv_heads, dim, dtype, n)
+        vr = _paged_rows(v, "v", kv_heads, dim, dtype, n)
+        half = 0 if inv_freq is None else inv_freq.numel()
+        if half & 7 or 2 * half > dim:
+            raise ValueError(f"inv_freq must have a multiple of 8 values, at most {dim // 2}")
+    else:
+        if kv_heads < 1 or heads % kv_heads:
+            raise ValueError("query heads must be a multiple of the kv heads")
+        if not softcap >= 0.0 or window < 0:
+            raise ValueError("softcap and window must be >= 0 (0: none)")
+        scale = dim ** -0.5 if scale is None else float(scale)
+        if not scale > 0.0:
+            raise ValueError("scale must be positive")
+        if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (n, heads)
+                                or not lse.is_contiguous()):
+            raise ValueError("lse must be contiguous fp32 [tokens, heads]")
+    if cu_q is None and n != batch:
+        raise ValueError("without cu_q there is one token per sequence of block_table")
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    if out.shape != like.shape or out.dtype != like.dtype:
-        raise ValueError(f"{name} must have the shape and type of q")
-    sn, sh, sd = out.stride()
-    if sd != 1 or sn % 8 or sh % 8 or out.data_ptr() % 16:
-        raise ValueError(f"{name}: contiguous head dimension, 16-byte aligned rows and heads")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        op, on, oh = out.data_ptr(), heads * dim, dim
+    else:
+        op, on, oh = _paged_rows(out, "out", heads, dim, dtype, n)
+    lib = _native.lib()
+    scratch = None
+    if k is None:
+        if cu_q is None:
+            need = lib.llmyb_paged_decode_scratch_bytes(heads, kv_heads, dim)
+        else:
+            need = lib.llmyb_paged_prefill_scratch_bytes(n, heads, kv_heads, dim, width, page_size)
+        if need > 0:
+            scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    f32 = torch.float32
+    args = _native.PAGED_ARGS.pack(
+        qp, kr[0], vr[0], _paged_vector(q_norm, "q_norm", f32, dim),
+        _paged_vector(k_norm, "k_norm", f32, dim), _paged_vector(inv_freq, "inv_freq", f32, half),
+        kp, vp, block_table.data_ptr(), lp, _paged_vector(cu_q, "cu_q", torch.int32, batch + 1),
+        _paged_vector(prefix, "prefix", torch.int32, batch),
+        _paged_vector(slopes, "slopes", f32, heads), op, 0 if lse is None else lse.data_ptr(),
+        0 if scratch is None else scratch.data_ptr(), device_status(q.device).data_ptr(), qn, qh,
+        kr[1], kr[2], vr[1], vr[2], on, oh, sp, sh, sr, st, n, batch, heads, kv_heads, dim,
+        dtype is torch.float16, pages, page_size, width, window, half, interleaved, scale, softcap,
+        eps, 0)
+    status = getattr(lib, entry)(args, torch._C._cuda_getCurrentRawStream(dev))
+    if status:
+        _native.check(status, entry)
     return out
-
-
-def _paged_lse(lse, like: torch.Tensor) -> None:
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != like.shape[:2]
-                            or not lse.is_contiguous()):
-        raise ValueError("lse must be contiguous fp32 [tokens, heads]")
-
-
-def _paged_scores(q, k_pages, scale, softcap, window, slopes) -> float:
-    if q.shape[1] % k_pages.shape[1]:
-        raise ValueError("query heads must be a multiple of the kv heads")
-    if not softcap >= 0.0 or window < 0:
-        raise ValueError("softcap and window must be >= 0 (0: none)")
-    _paged_f32(slopes, "slopes", q.shape[1])
-    scale = k_pages.shape[3] ** -0.5 if scale is None else float(scale)
-    if not scale > 0.0:
-        raise ValueError("scale must be positive")
-    return scale
 
 
 def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
@@ -1272,33 +1306,9 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     sequence) are the last positions of sequence b.  Rows behind cu_q[B] are
     left alone; a token at a negative position (a slot of length 0) is not
     stored and its query is zero.  q_out may be q."""
-    pool = _paged_pool(k_pages, v_pages, block_table, lengths, q, k, v, cu_q, inv_freq, q_norm,
-                       k_norm, q_out)
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        _paged_rows(t, name, k_pages)
-    n, heads, dim = q.shape
-    kv = k_pages.shape[1]
-    if k.shape != (n, kv, dim) or v.shape != (n, kv, dim):
-        raise ValueError(f"k and v must be [{n}, {kv}, {dim}]")
-    batch = lengths.shape[0]
-    if cu_q is not None:
-        _paged_i32(cu_q, "cu_q", batch + 1)
-    elif n != batch:
-        raise ValueError("without cu_q there is one token per sequence")
-    _paged_f32(q_norm, "q_norm", dim)
-    _paged_f32(k_norm, "k_norm", dim)
-    _paged_f32(inv_freq, "inv_freq")
-    half = 0 if inv_freq is None else inv_freq.shape[0]
-    if half % 8 or 2 * half > dim:
-        raise ValueError(f"inv_freq must have a multiple of 8 values, at most {dim // 2}")
-    q_out = _paged_out(q_out, q, "q_out")
-    _native.call("llmyb_paged_append", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
-                 k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), n, heads, kv,
-                 dim, k_pages.dtype is torch.float16, k_pages.data_ptr(), v_pages.data_ptr(),
-                 *pool, _ptr(cu_q), batch, _ptr(q_norm), _ptr(k_norm), eps, _ptr(inv_freq), half,
-                 interleaved, q_out.data_ptr(), q_out.stride(0), q_out.stride(1),
-                 device_status(q.device).data_ptr(), _stream())
-    return q_out
+    return _paged_call("llmyb_paged_append", q, k_pages, v_pages, block_table, lengths, q_out, k=k,
+                       v=v, cu_q=cu_q, inv_freq=inv_freq, interleaved=interleaved, q_norm=q_norm,
+                       k_norm=k_norm, eps=eps)
 
 
 def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -1313,23 +1323,8 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     at distance < window.  Query head h reads kv head h // (Hq / Hkv).  A
     sequence of length 0 gives zeros.  lse (fp32 [B, Hq]) receives the natural
     log-sum-exp of the scores."""
-    pool = _paged_pool(k_pages, v_pages, block_table, lengths, q, slopes, out, lse)
-    _paged_rows(q, "q", k_pages)
-    b, heads, dim = q.shape
-    kv = k_pages.shape[1]
-    if b != lengths.shape[0]:
-        raise ValueError("q must have one row per sequence of block_table")
-    scale = _paged_scores(q, k_pages, scale, softcap, window, slopes)
-    out = _paged_out(out, q)
-    _paged_lse(lse, q)
-    need = _native.lib().llmyb_paged_decode_scratch_bytes(heads, kv, dim)
-    scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _native.call("llmyb_paged_decode", q.data_ptr(), q.stride(0), q.stride(1), b, heads, kv, dim,
-                 k_pages.dtype is torch.float16, k_pages.data_ptr(), v_pages.data_ptr(), *pool,
-                 scale, softcap, window, _ptr(slopes), out.data_ptr(), out.stride(0),
-                 out.stride(1), _ptr(lse), scratch.data_ptr(), device_status(q.device).data_ptr(),
-                 _stream())
-    return out
+    return _paged_call("llmyb_paged_decode", q, k_pages, v_pages, block_table, lengths, out,
+                       scale=scale, softcap=softcap, window=window, slopes=slopes, lse=lse)
 
 
 def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -1345,27 +1340,10 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     (window > 0) or, instead of a window, also those j < prefix[b] (int32 [B]:
     a bidirectional prefix).  Rows that see no key give zeros; rows behind
     cu_q[B] are left alone.  lse: fp32 [N, Hq]."""
-    pool = _paged_pool(k_pages, v_pages, block_table, lengths, q, cu_q, slopes, prefix, out, lse)
-    _paged_rows(q, "q", k_pages)
-    n, heads, dim = q.shape
-    kv = k_pages.shape[1]
-    batch = lengths.shape[0]
-    _paged_i32(cu_q, "cu_q", batch + 1)
-    scale = _paged_scores(q, k_pages, scale, softcap, window, slopes)
-    if heads // kv > 128:
+    if prefix is not None and window:
+        raise ValueError("a prefix and a window exclude each other")
+    if q.shape[1] > 128 * k_pages.shape[1]:
         raise ValueError("at most 128 query heads per kv head")
-    if prefix is not None:
-        _paged_i32(prefix, "prefix", batch)
-        if window:
-            raise ValueError("a prefix and a window exclude each other")
-    out = _paged_out(out, q)
-    _paged_lse(lse, q)
-    need = _native.lib().llmyb_paged_prefill_scratch_bytes(n, heads, kv, dim, block_table.shape[1],
-                                                           k_pages.shape[2])
-    scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _native.call("llmyb_paged_prefill", q.data_ptr(), q.stride(0), q.stride(1), n, heads, kv, dim,
-                 k_pages.dtype is torch.float16, k_pages.data_ptr(), v_pages.data_ptr(), *pool,
-                 cu_q.data_ptr(), batch, _ptr(prefix), scale, softcap, window, _ptr(slopes),
-                 out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse), _ptr(scratch),
-                 device_status(q.device).data_ptr(), _stream())
-    return out
+    return _paged_call("llmyb_paged_prefill", q, k_pages, v_pages, block_table, lengths, out,
+                       cu_q=cu_q, scale=scale, softcap=softcap, window=window, slopes=slopes,
+                       prefix=prefix, lse=lse)

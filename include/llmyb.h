@@ -797,63 +797,66 @@ int32_t llmyb_decode_persistent(const llmyb_pdecode* p, void* stream);
  * cu_q[b] .. cu_q[b + 1) are the last cu_q[b+1] - cu_q[b] positions of
  * sequence b; rows behind cu_q[batch] are neither read nor written.  A page
  * number outside [0, num_pages) sets dev_status to LLMYB_EINVAL and is not
- * accessed.  Outputs must not overlap inputs, except q_out == q. */
+ * accessed.  Outputs must not overlap inputs, except out == q in append.
+ *
+ * The three calls take one argument block (host memory, read during the call);
+ * fields that a call does not name are ignored. */
+typedef struct {
+  const void* q;          /* [n_tokens][q_heads][head_dim] */
+  const void* k;          /* append: [n_tokens][kv_heads][head_dim] */
+  const void* v;
+  const float* q_norm;    /* append: [head_dim] or null */
+  const float* k_norm;
+  const float* inv_freq;  /* append: [rope_half] */
+  void* k_pages;
+  void* v_pages;
+  const int32_t* table;   /* [batch][table_width] */
+  const int32_t* lengths; /* [batch] */
+  const int32_t* cu_q;    /* [batch + 1] */
+  const int32_t* prefix;  /* prefill: [batch] or null */
+  const float* slopes;    /* attention: [q_heads] or null */
+  void* out;              /* [n_tokens][q_heads][head_dim] */
+  float* lse;             /* attention: [n_tokens][q_heads] or null */
+  void* scratch;          /* attention */
+  int32_t* dev_status;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
+      v_head_stride, out_token_stride, out_head_stride, page_stride, head_stride, row_stride,
+      table_stride;
+  int32_t n_tokens, batch, q_heads, kv_heads, head_dim, fp16, num_pages, page_size, table_width,
+      window, rope_half, interleaved;
+  float scale, softcap, eps;
+  int32_t reserved;       /* 0 */
+} llmyb_paged_args;
 
-/* q_out = rotate(norm(q)), pages <- rotate(norm(k)), v.  norm: x / sqrt(mean
- * x^2 + eps) * weight per head (q_norm / k_norm fp32 [head_dim], 16-byte
- * aligned, or null: none); rotate: by position * inv_freq[i], i < rope_half,
- * the pairs (x[i], x[i + rope_half]) or, interleaved, (x[2i], x[2i + 1]); the
- * dimensions behind 2 * rope_half pass (rope_half a multiple of 8, 0: none).
- * cu_q null: one token per sequence (n_tokens == batch).  A token whose
- * position is negative (length shorter than its tokens) is not stored and its
- * q_out row is zero. */
-int32_t llmyb_paged_append(
-    const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
-    int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
-    int64_t v_head_stride, int32_t n_tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
-    int32_t fp16, void* k_pages, void* v_pages, int64_t page_stride, int64_t head_stride,
-    int64_t row_stride, int32_t num_pages, int32_t page_size, const int32_t* table,
-    int64_t table_stride, int32_t table_width, const int32_t* lengths, const int32_t* cu_q,
-    int32_t batch, const float* q_norm, const float* k_norm, float eps, const float* inv_freq,
-    int32_t rope_half, int32_t interleaved, void* q_out, int64_t out_token_stride,
-    int64_t out_head_stride, int32_t* dev_status, void* stream);
+/* out = rotate(norm(q)), pages <- rotate(norm(k)), v.  norm: x / sqrt(mean
+ * x^2 + eps) * weight per head (q_norm / k_norm, 16-byte aligned, null: none);
+ * rotate: by position * inv_freq[i], i < rope_half, the pairs (x[i],
+ * x[i + rope_half]) or, interleaved, (x[2i], x[2i + 1]); the dimensions behind
+ * 2 * rope_half pass (rope_half a multiple of 8, 0: none).  cu_q null: one
+ * token per sequence (n_tokens == batch).  A token whose position is negative
+ * (length shorter than its tokens) is not stored and its out row is zero. */
+int32_t llmyb_paged_append(const llmyb_paged_args* args, void* stream);
 
-/* One token per sequence (row b of q, out; position lengths[b] - 1):
- * out = softmax(s) v over its visible keys, s = scale q.k (scale > 0), then
- * softcap * tanh(s / softcap) if softcap > 0, then - slopes[h] * distance if
- * slopes (fp32 [q_heads]); window > 0: distance < window.  A sequence of
- * length 0 gives zeros.  lse (or null) [batch][q_heads] fp32: natural log of
- * the sum of exp(s), -inf where no key is visible.  scratch: scratch_bytes of
- * the current device, not shared by calls that may run at the same time. */
+/* One token per sequence (n_tokens == batch; row b of q and out has position
+ * lengths[b] - 1): out = softmax(s) v over its visible keys, s = scale q.k
+ * (scale > 0), then softcap * tanh(s / softcap) if softcap > 0, then
+ * - slopes[h] * distance if slopes; window > 0: distance < window.  A sequence
+ * of length 0 gives zeros.  lse: natural log of the sum of exp(s), -inf where
+ * no key is visible.  scratch: scratch_bytes of the current device, not shared
+ * by calls that may run at the same time. */
 int64_t llmyb_paged_decode_scratch_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim);
-int32_t llmyb_paged_decode(
-    const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t batch, int32_t q_heads,
-    int32_t kv_heads, int32_t head_dim, int32_t fp16, const void* k_pages, const void* v_pages,
-    int64_t page_stride, int64_t head_stride, int64_t row_stride, int32_t num_pages,
-    int32_t page_size, const int32_t* table, int64_t table_stride, int32_t table_width,
-    const int32_t* lengths, float scale, float softcap, int32_t window, const float* slopes,
-    void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, void* scratch,
-    int32_t* dev_status, void* stream);
+int32_t llmyb_paged_decode(const llmyb_paged_args* args, void* stream);
 
 /* The packed tokens of a call (their keys and values already in the pages):
  * scores as in llmyb_paged_decode, key j visible from position i if j <= i and
- * (window > 0) i - j < window, or (prefix int32 [batch], not together with a
- * window) j < prefix[b].  Rows that see no key give zeros.  Values of visible
- * 128-key blocks must be finite (rows outside the sequence may hold anything).
- * q_heads / kv_heads <= 128.  lse (or null) [n_tokens][q_heads]; scratch may be
- * null where scratch_bytes is 0. */
+ * (window > 0) i - j < window, or (prefix, not together with a window)
+ * j < prefix[b].  Rows that see no key give zeros.  Values of visible 128-key
+ * blocks must be finite (rows outside the sequence may hold anything).
+ * q_heads / kv_heads <= 128; scratch may be null where scratch_bytes is 0. */
 int64_t llmyb_paged_prefill_scratch_bytes(int32_t n_tokens, int32_t q_heads, int32_t kv_heads,
                                           int32_t head_dim, int32_t table_width,
                                           int32_t page_size);
-int32_t llmyb_paged_prefill(
-    const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t n_tokens,
-    int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t fp16, const void* k_pages,
-    const void* v_pages, int64_t page_stride, int64_t head_stride, int64_t row_stride,
-    int32_t num_pages, int32_t page_size, const int32_t* table, int64_t table_stride,
-    int32_t table_width, const int32_t* lengths, const int32_t* cu_q, int32_t batch,
-    const int32_t* prefix, float scale, float softcap, int32_t window, const float* slopes,
-    void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, void* scratch,
-    int32_t* dev_status, void* stream);
+int32_t llmyb_paged_prefill(const llmyb_paged_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -131,7 +131,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "llmyb_paged_append": (I32, [C.c_char_p, P]),
     "llmyb_paged_decode_scratch_bytes": (I64, [I32, I32, I32]),
     "llmyb_paged_decode": (I32, [C.c_char_p, P]),
-    "llmyb_paged_prefill_scratch_bytes": (I64, [I32, I32, I32, I32, I32, I32]),
+    "llmyb_paged_prefill_scratch_bytes": (I64, [I32, I32, I32, I32, I32]),
     "llmyb_paged_prefill": (I32, [C.c_char_p, P]),
 }
 

@@ -82,9 +82,75 @@ __device__ __forceinline__ float tanh_exp(float x) {
   return 1.f - 2.f * fast_rcp(1.f + fast_exp2(x * (2.f * kLog2e)));
 }
 
-// log2 of the row's unnormalised weight sum -> natural log-sum-exp
+// natural log-sum-exp from the base-2 maximum and the weight sum (0: no key)
 __device__ __forceinline__ float lse_of(float m, float l) {
-  return l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+  return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// 1 / l, and 0 for a row without keys; a NaN stays one
+__device__ __forceinline__ float inv_of(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+// Two fp32 values in one 64-bit register: one issue slot for two operations.
+__device__ __forceinline__ uint64_t make2(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ float2 split2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// tanh of half of each value, |y| < 2: an odd polynomial, minimax fit of the
+// absolute error (2.2e-7).  The factor 1/2 makes "out of range" one bit of the
+// argument (2^1 and above, infinities and NaN have bit 30 set).
+__device__ __forceinline__ uint64_t tanh_half_poly2(uint64_t y) {
+  const uint64_t z = mul2(y, y);
+  auto c = [](double v) { return make2(static_cast<float>(v), static_cast<float>(v)); };
+  uint64_t p = fma2(z, c(-0.0028382681775838137 / 2048), c(0.016108887270092964 / 512));
+  p = fma2(z, p, c(-0.05096546933054924 / 128));
+  p = fma2(z, p, c(0.1325313001871109 / 32));
+  p = fma2(z, p, c(-0.3332393765449524 / 8));
+  p = fma2(z, p, c(0.9999968856 / 2));
+  return mul2(p, y);
+}
+
+// tanh of half of each value, any y: with x = y / 2 clamped to 7, x P(x^2) /
+// Q(x^2), minimax fit of the absolute error (9e-7; 1.7e-6 where clamped); one
+// reciprocal serves both: a/b and c/d are a d / (b d) and c b / (b d), Q in [1, 70].
+__device__ __forceinline__ uint64_t tanh_half2(uint64_t y) {
+  const float2 c = split2(y);
+  // the clamp drops a NaN, which would reach the other value by the reciprocal
+  const float lo = fminf(fmaxf(0.5f * c.x, -7.f), 7.f), hi = fminf(fmaxf(0.5f * c.y, -7.f), 7.f);
+  y = make2(lo, hi);
+  const uint64_t z = mul2(y, y);
+  uint64_t p = fma2(z, make2(3.9298196e-06f, 3.9298196e-06f), make2(0.0022769469f, 0.0022769469f));
+  p = fma2(z, p, make2(0.1230213613f, 0.1230213613f));
+  p = fma2(z, p, make2(0.9999956868f, 0.9999956868f));
+  p = mul2(p, y);
+  uint64_t q = fma2(z, make2(0.00014234632f, 0.00014234632f), make2(0.0210719839f, 0.0210719839f));
+  q = fma2(z, q, make2(0.4563398457f, 0.4563398457f));
+  q = fma2(z, q, make2(1.f, 1.f));
+  const float2 d = split2(q);
+  const float r = fast_rcp(d.x * d.y);
+  const float2 t = split2(mul2(mul2(p, make2(d.y, d.x)), make2(r, r)));
+  return make2(c.x == c.x ? t.x : c.x, c.y == c.y ? t.y : c.y);
 }
 
 inline int page_shift_of(int page_size) {

@@ -29,7 +29,6 @@ constexpr int kCtasPerSm = 2;
 constexpr int kStages = 3;
 constexpr int kStageBytes = 8192;  // keys 4 KB, values 4 KB
 constexpr int kSmem = kWarps * kStages * kStageBytes;
-constexpr int kJoinThreads = 128;
 
 struct DecodeArgs {
   const uint16_t* q;
@@ -334,7 +333,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) paged_decode_kernel(D
         for (int i = 0; i < 2; ++i) {
           const int r = r0 + 8 * i;
           if (r >= rows) continue;
-          const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
+          const float inv = inv_of(l[i]);
           uint16_t* dst = a.out + cu.b * a.o_tok + (head0 + r) * a.o_head + c0;
 #pragma unroll
           for (int n = 0; n < DH / 8; ++n)
@@ -370,14 +369,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) paged_decode_kernel(D
 }
 
 // Joins the pieces of the sequence-heads that several workers share: one CTA
-// per (sequence, kv head, chunk, row).
-template <typename T, int DH>
-__global__ void __launch_bounds__(kJoinThreads) paged_decode_join_kernel(DecodeArgs a) {
+// per (sequence, kv head, chunk, row), NT threads.
+template <typename T, int DH, int NT>
+__global__ void __launch_bounds__(NT) paged_decode_join_kernel(DecodeArgs a) {
   constexpr int KT = 2048 / DH;
   constexpr int kVec = DH / 4;                  // threads per part's row
-  constexpr int kLanes = kJoinThreads / kVec;   // parts read side by side
+  constexpr int kLanes = NT / kVec;   // parts read side by side
   __shared__ float4 s_o[kLanes][kVec];
-  __shared__ float s_red[kJoinThreads / 32][2];
+  __shared__ float s_red[NT / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = blockIdx.x % a.rows;
   const int seg = blockIdx.x / a.rows;
@@ -417,13 +416,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_decode_join_kernel(DecodeA
     return (2ll * w + (w == w0 && t0 > w0 * share ? 1 : 0)) * a.rows + r;
   };
   float m = -INFINITY;
-  for (int w = w0 + threadIdx.x; w <= w1; w += kJoinThreads) m = fmaxf(m, a.part_ml[at(w)].x);
+  for (int w = w0 + threadIdx.x; w <= w1; w += NT) m = fmaxf(m, a.part_ml[at(w)].x);
   m = warp_max(m);
-  if (lane == 0) s_red[warp][0] = m;
+  if (lane == 0) s_red[warp] = m;
   __syncthreads();
-  m = s_red[0][0];
+  m = s_red[0];
 #pragma unroll
-  for (int i = 1; i < kJoinThreads / 32; ++i) m = fmaxf(m, s_red[i][0]);
+  for (int i = 1; i < NT / 32; ++i) m = fmaxf(m, s_red[i]);
   const float base = m == -INFINITY ? 0.f : m;
   const int v = threadIdx.x % kVec, p = threadIdx.x / kVec;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -449,7 +448,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_decode_join_kernel(DecodeA
     o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
     l += s_l[i];
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = inv_of(l);
   uint16_t* dst = a.out + b * a.o_tok + head * a.o_head + 4 * v;
   *reinterpret_cast<uint2*>(dst) =
       make_uint2(Elem<T>::pack(o.x * inv, o.y * inv), Elem<T>::pack(o.z * inv, o.w * inv));
@@ -465,9 +464,14 @@ int32_t launch(const DecodeArgs& a, cudaStream_t s) {
   paged_decode_kernel<T, DH><<<a.workers / kWarps, kWarps * 32, kSmem, s>>>(a);
   st = launch_status();
   if (st) return st;
-  const int64_t join = static_cast<int64_t>(a.pool.batch) * a.pool.kv_heads * a.chunks * a.rows;
-  cudaError_t e = launch_pdl(paged_decode_join_kernel<T, DH>, dim3(static_cast<unsigned>(join)),
-                             dim3(kJoinThreads), 0, s, a);
+  // Pieces per row: with few rows there are many (one sequence, 4 kv heads:
+  // 296), which 128 threads would read one after another (29 us against 5).
+  const int64_t segments = static_cast<int64_t>(a.pool.batch) * a.pool.kv_heads * a.chunks;
+  const dim3 grid(static_cast<unsigned>(segments * a.rows));
+  const cudaError_t e =
+      a.workers > 16 * segments
+          ? launch_pdl(paged_decode_join_kernel<T, DH, 512>, grid, dim3(512), 0, s, a)
+          : launch_pdl(paged_decode_join_kernel<T, DH, 128>, grid, dim3(128), 0, s, a);
   count_launch(2);
   return e == cudaSuccess ? launch_status() : static_cast<int32_t>(e);
 }

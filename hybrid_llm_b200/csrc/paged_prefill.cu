@@ -11,22 +11,28 @@
 //
 // A tile is 128 rows = (128 / group) tokens x the group of query heads that
 // share a kv head, so keys and values are read once per group and a causal
-// tile wastes little on its diagonal.  A unit of work is two such tiles that
-// run in turn over the same 128-key blocks, from the diagonal down:
-//   warps 0-3, 4-7  softmax of tile 0 / 1 (one row per thread, TMEM lane = row):
-//                   scores from TMEM, mask on edge blocks, base-2 online softmax
-//                   with a lazily raised maximum (raised only past 2^8, O then
-//                   rescaled in TMEM), P in 16 bits over the scores' columns
+// tile wastes little on its diagonal.  A unit is two such tiles that run in
+// turn over the same 128-key blocks, from the diagonal down:
+//   warps 0-3, 4-7  softmax of tile 0 / 1 (one row per thread, TMEM lane = row)
 //   warp 8          TMA: queries once per unit, keys and values page by page in
 //                   one ring of 128-key blocks
 //   warp 9          MMA: O_t += P_t V then S_t = Q_t K of the next block, for
 //                   t = 0, 1: one tile's products run under the other's softmax
+// S in fp32 TMEM columns; P in 16 bits over S's first columns, the A operand of
+// the second product; O in fp32 TMEM, divided by the weight sum at the end.
+//
+// The key blocks of all units form one list that is cut into equal ranges, one
+// per CTA of a grid of one CTA per SM: prompts of any lengths load the SMs
+// alike, and one chunk behind a long context uses all of them.  A unit that a
+// range cuts leaves its unnormalised fp32 O, maxima and weight sums in scratch,
+// and a second launch joins them in a fixed order.
+//
 // Values of rows outside the sequence (behind its end, or before the window)
 // are zeroed in shared memory: they may hold anything, and a zero weight does
-// not cancel an infinity.  With few units the key axis of every unit is split
-// over several CTAs; their unnormalised fp32 sums are joined by a second launch.
-// All waits are bounded; a timeout records LLMYB_ETIMEOUT and every role unwinds.
+// not cancel an infinity.  All waits are bounded; a timeout records
+// LLMYB_ETIMEOUT and every role unwinds.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 #include "sm100.cuh"
@@ -35,138 +41,314 @@
 namespace llmyb {
 namespace {
 
-constexpr int kRows = 128;           // rows per tile = keys per block
-constexpr int kBox = kRows * 128;    // 128 rows x 64 elements
-constexpr int kThreads = 320;
+constexpr int kRows = 128;         // rows per tile = keys per block
+constexpr int kBox = kRows * 128;  // 128 rows x 64 elements
+constexpr int kThreads = 384;
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;  // 256 x 208 + 128 x 88 = 384 x 168
 constexpr uint32_t kTmemCols = 512;
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinRows = 32;
+// What a unit costs beside its blocks (queries, first scores, the output), in blocks.
+constexpr int kUnitCost = 3;
+// Positions of a range at least, so that a range begins inside a unit or holds
+// some of its blocks.
+constexpr int kMinRange = 5;
+// Up to this many blocks a unit is not cut: the second launch costs more.
+constexpr int kWholeBlocks = 4;
 
 template <int D>
 struct Layout {
   static constexpr int kTile = kRows * D * 2;
-  static constexpr int kStages = D == 128 ? 5 : 8;  // K and V blocks alternate
+  static constexpr int kStages = D == 128 ? 4 : 8;  // K and V blocks alternate
   static constexpr int kQ = 0;                      // two query tiles
   static constexpr int kKV = 2 * kTile;
-  static constexpr int kBar = kKV + kStages * kTile;
-  static constexpr int kSmem = kBar + 256 + 1024;   // + alignment slack
+  static constexpr int kOut = kKV + kStages * kTile;  // 4 KB per softmax warp
+  static constexpr int kBar = kOut + 8 * 4096;
+  static constexpr int kSmem = kBar + 512 + 1024;  // + alignment slack
+};
+
+// What a CTA leaves for the join: the cut unit that starts in its range, and
+// whether its range begins inside one.
+struct CutUnit {
+  int32_t slot;            // -1: none starts here
+  int32_t token, count;    // its first token and how many
+  int32_t kvh;
+  int32_t continues;       // the range begins inside a unit ...
+  int32_t ends;            // ... and holds that unit's last block
 };
 
 struct PrefillArgs {
   PagedPool pool;
   const int32_t* cu_q;
   const int32_t* prefix;  // or null
-  int32_t n_tokens, q_heads, group, tile_tokens, window, max_splits;
+  int32_t n_tokens, q_heads, group, tile_tokens, window;
+  int32_t cut;            // units may be cut
   float scale, softcap;
   const float* slopes;
   uint16_t* out;
   int64_t o_tok, o_head;
-  float* lse;      // [n_tokens, q_heads] or null
-  float* part_o;   // [splits][n_tokens][q_heads][D]
-  float2* part_ml; // [splits][n_tokens][q_heads]
+  float* lse;       // [n_tokens, q_heads] or null
+  float* part_o;    // [grid * 2][D / 4][256][4]
+  float2* part_ml;  // [grid * 2][256]
+  CutUnit* cuts;    // [grid]
   int32_t* dev_status;
 };
 
-// Tokens of sequence b: the first one and how many.
-__device__ __forceinline__ void tokens_of(const PrefillArgs& a, int b, int& q0, int& n) {
-  q0 = max(0, min(a.cu_q[b], a.n_tokens));
-  n = max(0, min(a.cu_q[b + 1], a.n_tokens) - q0);
-}
+struct Seq {
+  int q0, n, len, prefix;
 
-// (sequence, two-tile piece) pairs of the batch and the splits of each key
-// axis; by one warp.
-__device__ __forceinline__ int plan(const PrefillArgs& a, int grid, int& splits) {
-  const int lane = threadIdx.x & 31;
-  int sum = 0;
-  for (int b = lane; b < a.pool.batch; b += 32) {
-    int q0, n;
-    tokens_of(a, b, q0, n);
-    sum += (n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens);
+  __device__ __forceinline__ void load(const PrefillArgs& a, int b) {
+    q0 = max(0, min(a.cu_q[b], a.n_tokens));
+    n = max(0, min(a.cu_q[b + 1], a.n_tokens) - q0);
+    len = a.pool.length(b);
+    prefix = a.prefix ? max(0, min(a.prefix[b], len)) : 0;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const int units = sum * a.pool.kv_heads;
-  splits = max(1, min(a.max_splits, units > 0 ? grid / units : 1));
-  return units;
-}
-
-struct Unit {
-  int b, q0, n, t0;    // sequence, its first token, its tokens, first token of the unit
-  int kvh, split;
-  int len, pos;        // length; position of token t0
-  int lo, prefix;      // first key any row sees; prefix
-  int kb0, blocks;     // key blocks [kb0, kb0 + blocks)
-  int tiles;           // tiles with tokens: 1 or 2
+  __device__ __forceinline__ int pieces(const PrefillArgs& a) const {
+    return (n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens);
+  }
 };
 
-// Unit u of the grid; by one warp.
-__device__ __forceinline__ Unit unit_of(const PrefillArgs& a, int u, int splits) {
-  const int lane = threadIdx.x & 31;
-  const int per = a.pool.kv_heads * splits, step = 2 * a.tile_tokens;
-  Unit x;
-  x.b = 0;
-  int before = 0, pieces = 0;
-  for (int b0 = 0; b0 < a.pool.batch; b0 += 32) {
-    int mine = 0;
-    if (b0 + lane < a.pool.batch) {
-      int q0, n;
-      tokens_of(a, b0 + lane, q0, n);
-      mine = (n + step - 1) / step;
-    }
-    int inc = mine;
+// Key blocks [kb0, kb0 + count) that the tokens of one piece see.
+__device__ __forceinline__ int piece_blocks(const PrefillArgs& a, const Seq& s, int piece, int& kb0,
+                                            int& lo) {
+  const int t0 = piece * 2 * a.tile_tokens, pos = s.len - s.n + t0;
+  const int last = pos + min(2 * a.tile_tokens, s.n - t0) - 1;
+  int hi = last + 1;
+  if (last >= 0) hi = max(hi, s.prefix);
+  lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+  kb0 = lo / kRows;
+  return max(0, (hi + kRows - 1) / kRows - kb0);
+}
+
+// All pieces of the batch in order (sequence by sequence, last piece first),
+// in chunks of 32: one lane per piece.  A group is the pieces of 32 sequences.
+struct Group {
+  int b0;     // first sequence
+  Seq mine;   // of the lane's sequence
+  int inc;    // pieces up to and with it
+  int total;  // pieces of the group
+
+  __device__ __forceinline__ void load(const PrefillArgs& a, int first) {
+    const int lane = threadIdx.x & 31;
+    b0 = first;
+    mine = {0, 0, 0, 0};
+    if (b0 + lane < a.pool.batch) mine.load(a, b0 + lane);
+    inc = mine.pieces(a);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += y;
     }
-    const uint32_t hit = __ballot_sync(0xffffffffu, (before + inc) * per > u);
-    if (hit != 0) {
-      const int l = __ffs(hit) - 1;
-      x.b = b0 + l;
-      pieces = __shfl_sync(0xffffffffu, mine, l);
-      before += __shfl_sync(0xffffffffu, inc - mine, l);
-      break;
-    }
-    before += __shfl_sync(0xffffffffu, inc, 31);
+    total = __shfl_sync(0xffffffffu, inc, 31);
   }
-  const int r = u - before * per;
-  // the last tokens see the most keys: they start first
-  const int piece = pieces - 1 - r / per;
-  x.kvh = (r % per) / splits;
-  x.split = r % splits;
-  tokens_of(a, x.b, x.q0, x.n);
-  x.t0 = piece * step;
-  x.len = a.pool.length(x.b);
-  x.pos = x.len - x.n + x.t0;
-  const int count = min(step, x.n - x.t0);
-  x.tiles = count > a.tile_tokens ? 2 : 1;
-  x.prefix = a.prefix ? max(0, min(a.prefix[x.b], x.len)) : 0;
-  const int last = x.pos + count - 1;
-  int hi = last + 1;
-  if (last >= 0) hi = max(hi, x.prefix);
-  x.lo = a.window > 0 ? max(0, x.pos - a.window + 1) : 0;
-  const int kb0 = x.lo / kRows, nblk = max(0, (hi + kRows - 1) / kRows - kb0);
-  const int s0 = static_cast<int>(static_cast<int64_t>(nblk) * x.split / splits);
-  const int s1 = static_cast<int>(static_cast<int64_t>(nblk) * (x.split + 1) / splits);
-  x.kb0 = kb0 + s0;
-  x.blocks = s1 - s0;
-  return x;
+  // Of the lane's piece in the chunk from p0: its weight (0: none), sequence
+  // and number within it.
+  __device__ __forceinline__ int weight(const PrefillArgs& a, int p0, int& b, int& piece) const {
+    const int p = p0 + (threadIdx.x & 31);
+    int l = 0;  // first lane whose running count exceeds p
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      if (__shfl_sync(0xffffffffu, inc, l + o - 1) <= p) l += o;
+    const int end = __shfl_sync(0xffffffffu, inc, l);
+    Seq s;
+    s.q0 = 0;
+    s.n = __shfl_sync(0xffffffffu, mine.n, l);
+    s.len = __shfl_sync(0xffffffffu, mine.len, l);
+    s.prefix = __shfl_sync(0xffffffffu, mine.prefix, l);
+    b = b0 + l;
+    piece = end - 1 - p;  // end - pieces <= p < end
+    int kb0, lo;
+    return p < total ? (piece_blocks(a, s, piece, kb0, lo) + kUnitCost) * a.pool.kv_heads : 0;
+  }
+};
+
+// The range of one CTA and the unit that it begins in.
+struct Start {
+  int64_t begin, end;  // positions in the list of blocks and unit costs
+  int64_t at;          // position of the first unit
+  int b, piece, kvh;
+};
+
+// Before the roles part: every warp weighs some of the chunks into shared
+// memory, one warp looks the range's first unit up.  `sums` holds kSums chunk
+// sums; where a batch has more chunks (over 16,000 pieces), several share one.
+constexpr int kSums = 512;
+
+__device__ __forceinline__ Start find_start(const PrefillArgs& a, int64_t* sums, int warps) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // chunks at most: one per 32 pieces and one per group; pieces at most: one
+  // per unit's tokens and one per sequence
+  const int64_t pieces = a.n_tokens / (2 * a.tile_tokens) + a.pool.batch;
+  const int most = static_cast<int>(pieces / 32) + (a.pool.batch + 31) / 32 + 1;
+  const int per = (most + kSums - 1) / kSums;
+  for (int i = threadIdx.x; i < kSums; i += blockDim.x) sums[i] = 0;
+  __syncthreads();
+  Group g;
+  int chunk = 0;
+  for (int b0 = 0; b0 < a.pool.batch; b0 += 32) {
+    g.load(a, b0);
+    for (int p0 = 0; p0 < g.total; p0 += 32, ++chunk) {
+      if (chunk % warps != warp) continue;
+      int b, piece, w = g.weight(a, p0, b, piece);
+      w = __reduce_add_sync(0xffffffffu, w);
+      if (lane == 0) atomicAdd(reinterpret_cast<unsigned long long*>(&sums[min(chunk / per, kSums - 1)]),
+                  static_cast<unsigned long long>(w));
+    }
+  }
+  __syncthreads();
+  Start r = {0, 0, 0, a.pool.batch, 0, 0};
+  if (warp != 0) return r;
+  int64_t mine = 0;  // of kSums / 32 neighbours
+#pragma unroll
+  for (int i = 0; i < kSums / 32; ++i) mine += sums[lane * (kSums / 32) + i];
+  int64_t inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
+  }
+  const int64_t total = __shfl_sync(0xffffffffu, inc, 31);
+  // as many ranges as can have kMinRange positions (1 where units are not
+  // cut); the CTAs behind have none
+  const int64_t most_ranges = max(static_cast<int64_t>(1), a.cut ? total / kMinRange : total);
+  const int64_t ranges = min(static_cast<int64_t>(gridDim.x), most_ranges);
+  const int64_t c = min(static_cast<int64_t>(blockIdx.x), ranges);
+  r.begin = total * c / ranges;
+  r.end = total * min(c + 1, ranges) / ranges;
+  if (r.begin >= r.end) return r;
+  // the sum, then the chunk, then the piece that holds r.begin
+  const int l = __ffs(__ballot_sync(0xffffffffu, inc > r.begin)) - 1;
+  int64_t before = __shfl_sync(0xffffffffu, inc - mine, l);
+  int at = l * (kSums / 32);
+  while (before + sums[at] <= r.begin) before += sums[at++];
+  chunk = 0;
+  for (int b0 = 0; b0 < a.pool.batch; b0 += 32) {
+    g.load(a, b0);
+    const int chunks = (g.total + 31) / 32;
+    if (chunk + chunks > at * per) {
+      for (int k = max(0, at * per - chunk); k < chunks; ++k) {
+        int b, piece;
+        const int w = g.weight(a, 32 * k, b, piece);
+        int sum = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += y;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, before + sum > r.begin);
+        if (hit != 0) {
+          const int h = __ffs(hit) - 1;
+          r.b = __shfl_sync(0xffffffffu, b, h);
+          r.piece = __shfl_sync(0xffffffffu, piece, h);
+          const int unit = __shfl_sync(0xffffffffu, w, h) / a.pool.kv_heads;
+          before += __shfl_sync(0xffffffffu, sum - w, h);
+          r.kvh = static_cast<int>((r.begin - before) / unit);
+          r.at = before + static_cast<int64_t>(r.kvh) * unit;
+          return r;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+      }
+    }
+    chunk += chunks;
+  }
+  return r;
 }
 
-// i-th unit of this CTA: heavy units come first in the list, and every other
-// round runs backwards so that the rounds' differences cancel
-__device__ __forceinline__ int unit_index(int i) {
-  const int c = (i & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-  return i * gridDim.x + c;
+// A unit, or the part of it in one CTA's range, as the roles get it.
+struct Unit {
+  int blocks;         // key blocks [kb0, kb0 + blocks); -1: no more units
+  int kb0, tiles;     // tiles with tokens
+  int kvh;
+  int token, count;   // first token, how many
+  int pos;            // position of the first token
+  int prefix;
+  int starts, ends;   // the part holds the unit's last keys / first keys
+};
+
+// The units of one CTA's range, in order.
+struct Units {
+  Start at;  // the next unit
+  Seq s;
+  int b, lo;  // sequence of the current unit; first key any of its rows sees
+
+  __device__ __forceinline__ bool next(const PrefillArgs& a, Unit& u) {
+    while (at.at < at.end && at.b < a.pool.batch) {
+      if (at.piece < 0) {  // next sequence with tokens
+        if (++at.b == a.pool.batch) break;
+        s.load(a, at.b);
+        at.piece = s.pieces(a) - 1;
+        at.kvh = 0;
+        continue;
+      }
+      int kb0;
+      const int all = piece_blocks(a, s, at.piece, kb0, lo);
+      const int64_t here = at.at;
+      const int t0 = at.piece * 2 * a.tile_tokens;
+      at.at += all + kUnitCost;
+      b = at.b;
+      u.kvh = at.kvh;
+      if (++at.kvh == a.pool.kv_heads) {
+        at.kvh = 0;
+        --at.piece;
+      }
+      const bool first = here >= at.begin;  // the unit begins in this range
+      int s0 = 0, s1 = all;                 // its blocks, counted from the last keys
+      if (a.cut) {
+        if (!first) s0 = min(all, max(0, static_cast<int>(at.begin - here) - kUnitCost));
+        if (at.at > at.end) s1 = max(0, static_cast<int>(at.end - here) - kUnitCost);
+      } else if (!first) {
+        s1 = 0;
+      }
+      if (s0 >= s1 && !(all == 0 && first)) continue;
+      u.blocks = s1 - s0;
+      u.kb0 = kb0 + all - s1;
+      u.count = min(2 * a.tile_tokens, s.n - t0);
+      u.tiles = u.count > a.tile_tokens ? 2 : 1;
+      u.token = s.q0 + t0;
+      u.pos = s.len - s.n + t0;
+      u.prefix = s.prefix;
+      u.starts = s0 == 0;
+      u.ends = s1 == all;
+      return true;
+    }
+    return false;
+  }
+};
+
+// A wait that polls: the suspending wait of sm100.cuh wakes up to a
+// microsecond late, which the chain S -> P -> O pays twice per block
+// (prefill of 8192 tokens: 769 us with it, 614 us polling).  Bounded like it.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int32_t* status,
+                                     volatile int* abort_flag) {
+  for (int i = 0; i < 4096; ++i)
+    if (sm100::mbar_try_wait(bar, parity)) return true;
+  return sm100::mbar_wait_warp(bar, parity, status, abort_flag);
+}
+
+// elements e and e + 1 of a row of scores
+__device__ __forceinline__ uint64_t pair(const uint32_t (&s)[128], int e) {
+  return make2(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+}
+__device__ __forceinline__ void set_pair(uint32_t (&s)[128], int e, uint64_t v) {
+  const float2 x = split2(v);
+  s[e] = __float_as_uint(x.x);
+  s[e + 1] = __float_as_uint(x.y);
+}
+
+// largest of three, NaN if one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 template <typename T>
 constexpr uint32_t idesc(int n) {
   // D fp32; A and B bf16 (bits 7, 10) or fp16 (none)
   return sm100::make_idesc_bf16_f32(kRows, n) &
-         (sizeof(T) == 2 && std::is_same<T, __half>::value ? ~((1u << 7) | (1u << 10)) : ~0u);
+         (std::is_same<T, __half>::value ? ~((1u << 7) | (1u << 10)) : ~0u);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kCap, bool kBias>
 __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PrefillArgs a) {
@@ -183,18 +365,26 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
   uint64_t* s_full = bars + 4;      // [2]
   uint64_t* p_full = bars + 6;      // [2]
   uint64_t* o_full = bars + 8;      // [2]
-  uint64_t* kv_full = bars + 10;    // [kStages]
+  uint64_t* u_full = bars + 10;     // [2] units announced by the TMA warp
+  uint64_t* u_empty = bars + 12;    // [2]
+  uint64_t* kv_full = bars + 14;    // [kStages]
   uint64_t* kv_empty = kv_full + kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + kStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  Start* start = reinterpret_cast<Start*>(tmem_slot + 2);
+  Unit* ring = reinterpret_cast<Unit*>(start + 1);  // [2]
+  static_assert((14 + 2 * kStages) * 8 + 8 + sizeof(Start) + 2 * sizeof(Unit) <= 512, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
+  if (warp == 9) sm100::tmem_alloc(tmem_slot, kTmemCols);
+  if (threadIdx.x == 352) {
     for (int i = 0; i < 4; ++i) sm100::mbar_init(&bars[i], 1);
     for (int i = 0; i < 2; ++i) {
       sm100::mbar_init(&s_full[i], 1);
       sm100::mbar_init(&p_full[i], 4);  // one arrival per softmax warp
       sm100::mbar_init(&o_full[i], 1);
+      sm100::mbar_init(&u_full[i], 1);
+      sm100::mbar_init(&u_empty[i], 9);  // the softmax warps and the MMA warp
     }
     for (int i = 0; i < kStages; ++i) {
       sm100::mbar_init(&kv_full[i], 1);
@@ -206,173 +396,201 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
     sm100::tma_prefetch_desc(&map_k);
     sm100::tma_prefetch_desc(&map_v);
   }
-  if (warp == 9) sm100::tmem_alloc(tmem_slot, kTmemCols);
+  {
+    // the sums lie where the first queries will: order them before the copies
+    const Start r = find_start(a, reinterpret_cast<int64_t*>(smem + L::kQ), kThreads / 32);
+    if (threadIdx.x == 0) *start = r;
+    sm100::fence_proxy_async_smem();
+  }
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
   pdl_trigger();
   const uint32_t tmem = *tmem_slot;
   int32_t* const status = a.dev_status;
-  int splits;
-  const int units = plan(a, gridDim.x, splits) * splits;
+  if (a.cut && threadIdx.x == 0) a.cuts[blockIdx.x] = {-1, 0, 0, 0, 0, 0};
+  // the next unit, for every role but TMA's (n: units so far)
+  auto get = [&](uint32_t n, Unit& u) -> bool {
+    if (!wait(&u_full[n & 1], (n >> 1) & 1, status, abort_flag)) return false;
+    u = ring[n & 1];
+    __syncwarp();
+    if (lane == 0) sm100::mbar_arrive(&u_empty[n & 1]);
+    return u.blocks >= 0;
+  };
 
-  if (warp == 8) {
-    // ------------------------------------------------------------- TMA
-    uint32_t n_kv = 0, n_q = 0, n_raw = 0;
-    bool ok = true;
-    const int page_rows = min(1 << a.pool.page_shift, kRows);  // rows per copy
-    const int copies = kRows / page_rows * (D / 64);
-    // the lane's copy of a block: page piece and 64-element half
-    const int piece_row = lane / (D / 64) * page_rows, half = lane % (D / 64);
-    for (int i = 0; ok; ++i) {
-      const int u = unit_index(i);
-      if (i * static_cast<int>(gridDim.x) >= units) break;
-      if (u >= units) continue;
-      const Unit x = unit_of(a, u, splits);
-      if (x.blocks == 0) continue;
-      if (!(ok = sm100::mbar_wait_warp(q_empty, (n_q & 1) ^ 1u, status, abort_flag))) break;
-      if (lane == 0) {
-        const uint32_t rows = a.tile_tokens * a.group;
-        sm100::mbar_arrive_expect_tx(q_full, x.tiles * rows * D * 2);
-        for (int t = 0; t < x.tiles; ++t)
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-            sm100::tma_load_3d(&map_q, q_full, smem + L::kQ + t * L::kTile + c * kBox, c * 64,
-                               x.kvh * a.group, x.q0 + x.t0 + t * a.tile_tokens);
-      }
-      ++n_q;
-      const int32_t* row_table = a.pool.table + x.b * a.pool.table_stride;
-      for (int j = x.blocks - 1; j >= 0 && ok; --j) {
-        const int key0 = (x.kb0 + j) * kRows, key = key0 + piece_row;
-        const bool held = lane < copies && key < x.len && key + page_rows > x.lo;
-        int page = 0;
-        if (held) {
-          page = row_table[key >> a.pool.page_shift];
-          if (page < 0 || page >= a.pool.num_pages) {
-            report_status(status, LLMYB_EINVAL);
-            page = 0;
-          }
+  // the register split is set inside the role branches: what follows a common
+  // point would be compiled for the smaller share
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 8) {
+      // ----------------------------------------------------------- TMA
+      uint32_t n_kv = 0, n_q = 0, n_raw = 0;
+      bool ok = true;
+      const int page_rows = min(1 << a.pool.page_shift, kRows);  // rows per copy
+      const int copies = kRows / page_rows * (D / 64);
+      // the lane's copy of a block: page piece and 64-element half
+      const int piece_row = lane / (D / 64) * page_rows, half = lane % (D / 64);
+      Units x;
+      x.at = *start;
+      if (x.at.b < a.pool.batch) x.s.load(a, x.at.b);
+      for (uint32_t n = 0; ok; ++n) {
+        Unit u;
+        if (!x.next(a, u)) u.blocks = -1;
+        if (!(ok = wait(&u_empty[n & 1], ((n >> 1) & 1) ^ 1u, status, abort_flag))) break;
+        if (lane == 0) {
+          ring[n & 1] = u;
+          sm100::mbar_arrive(&u_full[n & 1]);
         }
-        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, held)) * page_rows * 128;
-        const int in_page = key & ((1 << a.pool.page_shift) - 1);
-        const bool mend = key0 + kRows > x.len || key0 < x.lo;
+        __syncwarp();
+        if (u.blocks < 0) break;
+        const int blocks = u.blocks, kb0 = u.kb0, len = x.s.len, lo = x.lo, kvh = u.kvh;
+        if (blocks == 0) continue;
+        if (!(ok = wait(q_empty, (n_q & 1) ^ 1u, status, abort_flag))) break;
+        if (lane == 0) {
+          sm100::mbar_arrive_expect_tx(q_full, u.tiles * a.tile_tokens * a.group * D * 2);
+          for (int t = 0; t < u.tiles; ++t)
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const uint32_t s = n_kv % kStages, ph = (n_kv / kStages) & 1;
-          if (!(ok = sm100::mbar_wait_warp(&kv_empty[s], ph ^ 1u, status, abort_flag))) break;
-          uint8_t* dst = smem + L::kKV + s * L::kTile;
-          uint64_t* bar = kv == 1 && mend ? v_raw : &kv_full[s];
-          if (lane == 0) sm100::mbar_arrive_expect_tx(bar, bytes);
-          __syncwarp();
-          if (held)
-            sm100::tma_load_4d(kv == 0 ? &map_k : &map_v, bar, dst + half * kBox + piece_row * 128,
-                               half * 64, in_page, x.kvh, page);
-          ++n_kv;
-          if (kv == 1 && mend) {
-            if (!(ok = sm100::mbar_wait_warp(v_raw, n_raw & 1, status, abort_flag))) break;
-            ++n_raw;
-            const int r0 = max(0, x.lo - key0), r1 = max(0, min(kRows, x.len - key0));
-            for (int k = lane; k < kRows * 8 * (D / 64); k += 32) {
-              const int r = (k >> 3) & (kRows - 1);
-              if (r < r0 || r >= r1)
-                *reinterpret_cast<uint4*>(dst + (k >> 10) * kBox + r * 128 + (k & 7) * 16) =
-                    make_uint4(0, 0, 0, 0);
+            for (int c = 0; c < D / 64; ++c)
+              sm100::tma_load_3d(&map_q, q_full, smem + L::kQ + t * L::kTile + c * kBox, c * 64,
+                                 kvh * a.group, u.token + t * a.tile_tokens);
+        }
+        ++n_q;
+        const int32_t* row_table = a.pool.table + x.b * a.pool.table_stride;
+        for (int j = blocks - 1; j >= 0 && ok; --j) {
+          const int key0 = (kb0 + j) * kRows, key = key0 + piece_row;
+          const bool held = lane < copies && key < len && key + page_rows > lo;
+          int page = 0;
+          if (held) {
+            page = row_table[key >> a.pool.page_shift];
+            if (page < 0 || page >= a.pool.num_pages) {
+              report_status(status, LLMYB_EINVAL);
+              page = 0;
             }
-            sm100::fence_proxy_async_smem();
+          }
+          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, held)) * page_rows * 128;
+          const int in_page = key & ((1 << a.pool.page_shift) - 1);
+          const bool mend = key0 + kRows > len || key0 < lo;
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            const uint32_t s = n_kv % kStages, ph = (n_kv / kStages) & 1;
+            if (!(ok = wait(&kv_empty[s], ph ^ 1u, status, abort_flag))) break;
+            uint8_t* dst = smem + L::kKV + s * L::kTile;
+            uint64_t* bar = kv == 1 && mend ? v_raw : &kv_full[s];
+            if (lane == 0) sm100::mbar_arrive_expect_tx(bar, bytes);
             __syncwarp();
-            if (lane == 0) sm100::mbar_arrive(&kv_full[s]);
-          }
-        }
-      }
-    }
-    // no copy into shared memory may still be in flight at exit (after a
-    // timeout; otherwise every one of these has been waited for)
-    if (!ok) {
-      if (n_q > 0) sm100::mbar_wait_warp(q_full, (n_q - 1) & 1, status, nullptr);
-      for (uint32_t i = 1; i <= kStages && i <= n_kv; ++i)
-        sm100::mbar_wait_warp(&kv_full[(n_kv - i) % kStages], ((n_kv - i) / kStages) & 1, status,
-                              nullptr);
-    }
-  } else if (warp == 9) {
-    // ------------------------------------------------------ MMA issuer
-    constexpr uint32_t idesc_s = idesc<T>(kRows);
-    constexpr uint32_t idesc_o = idesc<T>(D) | sm100::kIdescBMajorMN;
-    const uint32_t q_addr = sm100::smem_u32(smem + L::kQ);
-    const uint32_t kv_addr = sm100::smem_u32(smem + L::kKV);
-    uint32_t n_kv = 0, n_q = 0, n_p[2] = {0, 0};
-    bool ok = true;
-    auto wait_kv = [&](uint32_t n) {
-      return sm100::mbar_wait_warp(&kv_full[n % kStages], (n / kStages) & 1, status, abort_flag);
-    };
-    auto issue_s = [&](int t, uint32_t n) {  // S_t = Q_t K^T, K in load n
-      if (lane == 0) {
-        const uint32_t qa = q_addr + t * L::kTile, ka = kv_addr + (n % kStages) * L::kTile;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kBox + (kk & 3) * 32;
-          sm100::umma_bf16_ss(tmem + t * 128, sm100::make_sw128_kmajor_desc(qa + off),
-                              sm100::make_sw128_kmajor_desc(ka + off), idesc_s, kk > 0 ? 1u : 0u);
-        }
-        sm100::umma_commit(&s_full[t]);
-      }
-      __syncwarp();
-    };
-    auto issue_pv = [&](int t, uint32_t n, bool first) {  // O_t (+)= P_t V, V in load n
-      if (lane == 0) {
-        const uint32_t va = kv_addr + (n % kStages) * L::kTile;
-#pragma unroll
-        for (int kk = 0; kk < kRows / 16; ++kk)
-          sm100::umma_bf16_ts(tmem + 256 + t * D, tmem + t * 128 + kk * 8,
-                              sm100::make_sw128_desc(va + kk * 2048, kBox, 1024), idesc_o,
-                              (first && kk == 0) ? 0u : 1u);
-      }
-      __syncwarp();
-    };
-    auto commit = [&](uint64_t* bar) {
-      if (lane == 0) sm100::umma_commit(bar);
-      __syncwarp();
-    };
-    for (int i = 0; ok; ++i) {
-      const int u = unit_index(i);
-      if (i * static_cast<int>(gridDim.x) >= units) break;
-      if (u >= units) continue;
-      const Unit x = unit_of(a, u, splits);
-      if (x.blocks == 0) continue;
-      if (!(ok = sm100::mbar_wait_warp(q_full, n_q & 1, status, abort_flag) && wait_kv(n_kv)))
-        break;
-      ++n_q;
-      sm100::tc_fence_after();
-      for (int t = 0; t < x.tiles; ++t) issue_s(t, n_kv);
-      commit(&kv_empty[n_kv % kStages]);
-      if (x.blocks == 1) commit(q_empty);
-      for (int j = 0; j < x.blocks && ok; ++j) {
-        // load n_kv is the keys of block j, n_kv + 1 its values
-        const bool more = j + 1 < x.blocks;
-        if (!(ok = wait_kv(n_kv + 1))) break;
-        for (int t = 0; t < x.tiles; ++t) {
-          if (!(ok = sm100::mbar_wait_warp(&p_full[t], n_p[t] & 1, status, abort_flag))) break;
-          ++n_p[t];
-          sm100::tc_fence_after();
-          issue_pv(t, n_kv + 1, j == 0);
-          if (t == x.tiles - 1) commit(&kv_empty[(n_kv + 1) % kStages]);
-          if (more) {
-            if (t == 0 && !(ok = wait_kv(n_kv + 2))) break;
-            issue_s(t, n_kv + 2);
-            if (t == x.tiles - 1) {
-              commit(&kv_empty[(n_kv + 2) % kStages]);
-              if (j + 2 == x.blocks) commit(q_empty);
+            if (held)
+              sm100::tma_load_4d(kv == 0 ? &map_k : &map_v, bar, dst + half * kBox + piece_row * 128,
+                                 half * 64, in_page, kvh, page);
+            ++n_kv;
+            if (kv == 1 && mend) {
+              if (!(ok = wait(v_raw, n_raw & 1, status, abort_flag))) break;
+              ++n_raw;
+              const int r0 = max(0, lo - key0), r1 = max(0, min(kRows, len - key0));
+              for (int k = lane; k < kRows * 8 * (D / 64); k += 32) {
+                const int r = (k >> 3) & (kRows - 1);
+                if (r < r0 || r >= r1)
+                  *reinterpret_cast<uint4*>(dst + (k >> 10) * kBox + r * 128 + (k & 7) * 16) =
+                      make_uint4(0, 0, 0, 0);
+              }
+              sm100::fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) sm100::mbar_arrive(&kv_full[s]);
             }
-          } else {
-            commit(&o_full[t]);
           }
         }
-        n_kv += 2;
       }
+      // no copy into shared memory may still be in flight at exit (after a
+      // timeout; otherwise every one of these has been waited for)
+      if (!ok) {
+        if (n_q > 0) wait(q_full, (n_q - 1) & 1, status, nullptr);
+        for (uint32_t i = 1; i <= kStages && i <= n_kv; ++i)
+          wait(&kv_full[(n_kv - i) % kStages], ((n_kv - i) / kStages) & 1, status, nullptr);
+      }
+    } else if (warp == 9) {
+      // ---------------------------------------------------- MMA issuer
+      constexpr uint32_t idesc_s = idesc<T>(kRows);
+      constexpr uint32_t idesc_o = idesc<T>(D) | sm100::kIdescBMajorMN;
+      // This warp shares its scheduler with softmax warps and issues a product
+      // every 64 cycles, so its instructions count: one elected thread issues
+      // (with lane == 0 in its place the operands went through per-thread
+      // registers: 609 us against 558), and descriptors are made once, tiles
+      // and steps differing in the address field alone (538 us against 484;
+      // shared memory ends below 2^18, so the field does not overflow).
+      const uint64_t q_desc = sm100::make_sw128_kmajor_desc(sm100::smem_u32(smem + L::kQ));
+      const uint64_t k_desc = sm100::make_sw128_kmajor_desc(sm100::smem_u32(smem + L::kKV));
+      const uint64_t v_desc = sm100::make_sw128_desc(sm100::smem_u32(smem + L::kKV), kBox, 1024);
+      uint32_t n_kv = 0, n_q = 0, n_p[2] = {0, 0};
+      bool ok = true;
+      auto wait_kv = [&](uint32_t n) {
+        return wait(&kv_full[n % kStages], (n / kStages) & 1, status, abort_flag);
+      };
+      auto issue_s = [&](int t, uint32_t n) {  // S_t = Q_t K^T, K in load n
+        if (sm100::elect_one()) {
+          const uint64_t qd = q_desc + t * (L::kTile >> 4);
+          const uint64_t kd = k_desc + (n % kStages) * (L::kTile >> 4);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
+            sm100::umma_bf16_ss(tmem + t * 128, qd + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+          }
+          sm100::umma_commit(&s_full[t]);
+        }
+        __syncwarp();
+      };
+      auto issue_pv = [&](int t, uint32_t n, bool first) {  // O_t (+)= P_t V, V in load n
+        if (sm100::elect_one()) {
+          const uint64_t vd = v_desc + (n % kStages) * (L::kTile >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kRows / 16; ++kk)
+            sm100::umma_bf16_ts(tmem + 256 + t * D, tmem + t * 128 + kk * 8,
+                                vd + kk * (2048 >> 4), idesc_o, (first && kk == 0) ? 0u : 1u);
+        }
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (sm100::elect_one()) sm100::umma_commit(bar);
+        __syncwarp();
+      };
+      Unit u;
+      for (uint32_t n = 0; ok && get(n, u); ++n) {
+        const int blocks = u.blocks, tiles = u.tiles;
+        if (blocks == 0) continue;
+        if (!(ok = wait(q_full, n_q & 1, status, abort_flag) && wait_kv(n_kv))) break;
+        ++n_q;
+        sm100::tc_fence_after();
+        for (int t = 0; t < tiles; ++t) issue_s(t, n_kv);
+        commit(&kv_empty[n_kv % kStages]);
+        if (blocks == 1) commit(q_empty);
+        for (int j = 0; j < blocks && ok; ++j) {
+          // load n_kv is the keys of block j, n_kv + 1 its values
+          const bool more = j + 1 < blocks;
+          if (!(ok = wait_kv(n_kv + 1))) break;
+          for (int t = 0; t < tiles; ++t) {
+            if (!(ok = wait(&p_full[t], n_p[t] & 1, status, abort_flag))) break;
+            ++n_p[t];
+            sm100::tc_fence_after();
+            issue_pv(t, n_kv + 1, j == 0);
+            if (t == tiles - 1) commit(&kv_empty[(n_kv + 1) % kStages]);
+            if (more) {
+              if (t == 0 && !(ok = wait_kv(n_kv + 2))) break;
+              issue_s(t, n_kv + 2);
+              if (t == tiles - 1) {
+                commit(&kv_empty[(n_kv + 2) % kStages]);
+                if (j + 2 == blocks) commit(q_empty);
+              }
+            } else {
+              commit(&o_full[t]);
+            }
+          }
+          n_kv += 2;
+        }
+      }
+      // every MMA completes before TMEM and shared memory go away
+      commit(mma_done);
+      wait(mma_done, 0, status, nullptr);
     }
-    // every MMA completes before TMEM and shared memory go away
-    commit(mma_done);
-    sm100::mbar_wait_warp(mma_done, 0, status, nullptr);
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // --------------------------------------------------------- softmax
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -380,110 +598,161 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
     const int tok = row / a.group, g = row % a.group;  // token and head within the tile
     uint32_t n_s = 0, n_o = 0;
     bool ok = true;
-    for (int i = 0; ok; ++i) {
-      const int u = unit_index(i);
-      if (i * static_cast<int>(gridDim.x) >= units) break;
-      if (u >= units) continue;
-      const Unit x = unit_of(a, u, splits);
-      if (t >= x.tiles) continue;
-      const int local = x.t0 + t * a.tile_tokens + tok;
-      const bool live = tok < a.tile_tokens && local < x.n;
-      const int head = x.kvh * a.group + g;
-      const int pos = x.len - x.n + local;
+    Unit u;
+    for (uint32_t n = 0; ok && get(n, u); ++n) {
+      const bool whole = u.starts && u.ends;
+      if (threadIdx.x == 0 && !whole) {
+        CutUnit& cut = a.cuts[blockIdx.x];
+        if (u.starts) {
+          cut.slot = 1, cut.token = u.token, cut.count = u.count, cut.kvh = u.kvh;
+        } else {
+          cut.continues = 1, cut.ends = u.ends;
+        }
+      }
+      if (t >= u.tiles) continue;
+      const int local = t * a.tile_tokens + tok;  // within the unit
+      const bool live = tok < a.tile_tokens && local < u.count;
+      const int pos = u.pos + local;
       // visible keys of this row: lo <= j <= hi
       const int lo = a.window > 0 ? pos - a.window + 1 : 0;
-      const int hi = pos < 0 ? -1 : max(pos, x.prefix - 1);
+      const int hi = pos < 0 ? -1 : max(pos, u.prefix - 1);
       // of every row of the tile: max lo, min hi
-      const int first_pos = x.pos + t * a.tile_tokens;
-      const int tile_hi = first_pos < 0 ? -1 : max(first_pos, x.prefix - 1);
+      const int first_pos = u.pos + t * a.tile_tokens;
+      const int tile_hi = first_pos < 0 ? -1 : max(first_pos, u.prefix - 1);
       const int tile_lo = a.window > 0 ? first_pos + a.tile_tokens - a.window : 0;
-      const float slope = a.slopes && live ? a.slopes[head] * kLog2e : 0.f;
+      const float slope = kBias && live ? a.slopes[u.kvh * a.group + g] * kLog2e : 0.f;
+      // l: this row's weights by 2^-m; settled: every live row of the warp has
+      // its first maximum
       float m = -INFINITY, l = 0.f;
-      for (int j = x.blocks - 1; j >= 0; --j) {
-        if (!(ok = sm100::mbar_wait_warp(&s_full[t], n_s & 1, status, abort_flag))) break;
+      bool settled = false;
+      const int blocks = u.blocks, kb0 = u.kb0;
+      for (int j = blocks - 1; j >= 0; --j) {
+        if (!(ok = wait(&s_full[t], n_s & 1, status, abort_flag))) break;
         ++n_s;
         sm100::tc_fence_after();
-        uint32_t sr[4][32];
+        uint32_t sr[128];
+        {
+          uint32_t part[4][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) sm100::tmem_ld_32x32b_x32(t_s + 32 * c, sr[c]);
-        sm100::tmem_ld_wait();
+          for (int c = 0; c < 4; ++c) sm100::tmem_ld_32x32b_x32(t_s + 32 * c, part[c]);
+          sm100::tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) sm100::tmem_regs_ready(sr[c]);
-        const int j0 = (x.kb0 + j) * kRows;
+          for (int c = 0; c < 4; ++c) sm100::tmem_regs_ready(part[c]);
+#pragma unroll
+          for (int e = 0; e < 128; ++e) sr[e] = part[e / 32][e % 32];
+        }
+        const int j0 = (kb0 + j) * kRows;
         float sc = a.scale * kLog2e;
-        if (a.softcap > 0.f) {
-          const float in = a.scale / a.softcap, outer = a.softcap * kLog2e;
+        if constexpr (kCap) {
+          // cap tanh(s / cap): the short form while |s| < cap, which one bit of
+          // 2 s / cap tells
+          const float in = 2.f * a.scale / a.softcap;
+          const uint64_t in2 = make2(in, in);
+          uint32_t big = 0u;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int e = 0; e < 128; e += 2) {
+            set_pair(sr, e, mul2(pair(sr, e), in2));
+            big |= sr[e] | sr[e + 1];
+          }
+          if (__builtin_expect(__any_sync(0xffffffffu, big & 0x40000000u), 0)) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              sr[c][e] = __float_as_uint(outer * tanh_exp(__uint_as_float(sr[c][e]) * in));
-          sc = 1.f;
+            for (int e = 0; e < 128; e += 2) set_pair(sr, e, tanh_half2(pair(sr, e)));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 128; e += 2) set_pair(sr, e, tanh_half_poly2(pair(sr, e)));
+          }
+          sc = a.softcap * kLog2e;
         }
-        if (a.slopes) {
+        if constexpr (kBias) {
           const float d0 = static_cast<float>(pos - j0);
+          if (u.prefix == 0 || j0 + kRows - 1 <= first_pos) {  // no visible key is ahead
+            const uint64_t step = make2(slope, slope), sc2 = make2(sc, sc);
+            const uint64_t b0 = make2(-slope * d0, -slope * d0);
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+            for (int e = 0; e < 128; e += 2)
+              set_pair(sr, e,
+                       fma2(pair(sr, e), sc2,
+                            fma2(step, make2(static_cast<float>(e), static_cast<float>(e + 1)), b0)));
+          } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              sr[c][e] = __float_as_uint(fmaf(-slope, fabsf(d0 - (32 * c + e)),
-                                              __uint_as_float(sr[c][e]) * sc));
+            for (int e = 0; e < 128; ++e)
+              sr[e] = __float_as_uint(fmaf(-slope, fabsf(d0 - e), __uint_as_float(sr[e]) * sc));
+          }
           sc = 1.f;
         }
-        if (j0 + kRows - 1 > tile_hi || j0 < tile_lo) {
+        if (__builtin_expect(j0 + kRows - 1 > tile_hi || j0 < tile_lo, 0)) {
           const int lo_c = lo - j0, hi_c = hi - j0;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (32 * c + e < lo_c || 32 * c + e > hi_c) sr[c][e] = __float_as_uint(-INFINITY);
+          for (int e = 0; e < 128; ++e)
+            if (e < lo_c || e > hi_c) sr[e] = __float_as_uint(-INFINITY);
         }
-        float mx[8];
+        auto raise = [&]() {  // m to the block's maximum, l and O rescaled
+          float mx[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mx[e] = -INFINITY;
+          for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sr[e]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+          for (int e = 4; e < 124; e += 8)
 #pragma unroll
-          for (int e = 0; e < 32; ++e) mx[e & 7] = fmaxf(mx[e & 7], __uint_as_float(sr[c][e]));
-        const float bm = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
-                               fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * sc;
-        const bool raise = bm > m + 8.f;
-        float alpha = 1.f;
-        if (raise) {
-          alpha = fast_exp2(m - bm);
-          l *= alpha;
-          m = bm;
-        }
-        if (__any_sync(0xffffffffu, raise) && j != x.blocks - 1) {
-          // the scores of this block were issued behind the previous block's
-          // product, so O is complete
+            for (int k = 0; k < 4; ++k)
+              mx[k] = max3(mx[k], __uint_as_float(sr[e + 2 * k]), __uint_as_float(sr[e + 2 * k + 1]));
+          mx[0] = max3(mx[0], __uint_as_float(sr[124]), __uint_as_float(sr[125]));
+          mx[1] = max3(mx[1], __uint_as_float(sr[126]), __uint_as_float(sr[127]));
+          const float bm = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * sc;
+          float alpha = 1.f;
+          if (bm > m) {
+            alpha = fast_exp2(m - bm);
+            m = bm;
+            l *= alpha;
+          }
+          if (j != blocks - 1) {
+            // the scores of this block were issued behind the previous block's
+            // product, so O is complete
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            sm100::tmem_ld_32x32b_x32(t_o + 32 * c, o);
-            sm100::tmem_ld_wait();
-            sm100::tmem_regs_ready(o);
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              sm100::tmem_ld_32x32b_x32(t_o + 32 * c, o);
+              sm100::tmem_ld_wait();
+              sm100::tmem_regs_ready(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            sm100::tmem_st_32x32b_x32(t_o + 32 * c, o);
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              sm100::tmem_st_32x32b_x32(t_o + 32 * c, o);
+            }
           }
-        }
-        const float base = m == -INFINITY ? 0.f : -m;
-        float rs[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        };
+        auto weights = [&]() -> float {  // P = 2^(s - m) to TMEM, and its row sum
+          const float base = m == -INFINITY ? 0.f : -m;
+          const uint64_t sc2 = make2(sc, sc), base2 = make2(base, base);
+          uint64_t rs[2] = {0ull, 0ull};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t p[16];
+          for (int c = 0; c < 4; ++c) {
+            uint32_t p[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float p0 = fast_exp2(fmaf(__uint_as_float(sr[c][2 * e]), sc, base));
-            const float p1 = fast_exp2(fmaf(__uint_as_float(sr[c][2 * e + 1]), sc, base));
-            rs[(2 * e) & 7] += p0;
-            rs[(2 * e + 1) & 7] += p1;
-            p[e] = Elem<T>::pack(p0, p1);
+            for (int e = 0; e < 16; ++e) {
+              float2 w = split2(fma2(pair(sr, 32 * c + 2 * e), sc2, base2));
+              w.x = fast_exp2(w.x), w.y = fast_exp2(w.y);
+              rs[e & 1] = add2(rs[e & 1], make2(w.x, w.y));
+              p[e] = Elem<T>::pack(w.x, w.y);
+            }
+            sm100::tmem_st_32x32b_x16(t_s + 16 * c, p);
           }
-          sm100::tmem_st_32x32b_x16(t_s + 16 * c, p);
+          const float2 r = split2(add2(rs[0], rs[1]));
+          return r.x + r.y;
+        };
+        // The weights take the maximum of the blocks before.  Their sum shows
+        // whether that is still near enough: below 2^14 every one is (fp16
+        // holds 2^16, sums are fp32), and the block's own maximum is never
+        // formed (459 us against 502 with it).  Else, a NaN among them
+        // included, and at a row's first keys it is.
+        if (!settled) {
+          if (__any_sync(0xffffffffu, live && m == -INFINITY && hi >= j0)) raise();
+          settled = __all_sync(0xffffffffu, !live || m != -INFINITY);
         }
-        l += ((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]));
+        float sum = weights();
+        if (__builtin_expect(__any_sync(0xffffffffu, !(sum <= 16384.f)), 0)) {
+          raise();
+          sum = weights();
+        }
+        l += sum;
         sm100::tmem_st_wait();
         sm100::tc_fence_before();
         __syncwarp();
@@ -491,18 +760,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
       }
       if (!ok) break;
       // ---------------------------------------------------- epilogue
-      if (x.blocks > 0) {
-        if (!(ok = sm100::mbar_wait_warp(&o_full[t], n_o & 1, status, abort_flag))) break;
+      if (blocks > 0) {
+        if (!(ok = wait(&o_full[t], n_o & 1, status, abort_flag))) break;
         ++n_o;
         sm100::tc_fence_after();
       }
-      const int64_t token = x.q0 + local;
-      const int64_t at = (static_cast<int64_t>(x.split) * a.n_tokens + token) * a.q_heads + head;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = inv_of(l);
+      const int head = u.kvh * a.group + g;
+      // This row's place in the output; the rows go there by way of shared
+      // memory, 64 columns at a time, so that a store instruction writes whole
+      // 128-byte lines (one row per thread: four times as long).
+      const int64_t dst = live ? static_cast<int64_t>(u.token + local) * a.o_tok + head * a.o_head : -1;
+      uint8_t* const stage = smem + L::kOut + warp * 4096;
+      float4* const part = reinterpret_cast<float4*>(a.part_o) +
+                           (2ll * blockIdx.x + (u.starts ? 1 : 0)) * (256 * D / 4) + t * kRows + row;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
-        if (x.blocks > 0) {
+        if (blocks > 0) {
           sm100::tmem_ld_32x32b_x32(t_o + 32 * c, o);
           sm100::tmem_ld_wait();
           sm100::tmem_regs_ready(o);
@@ -510,29 +785,40 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0u;
         }
-        if (!live) continue;
-        if (splits > 1) {
-          float4* dst = reinterpret_cast<float4*>(a.part_o + at * D + 32 * c);
+        if (!whole) {  // column quads by row: the lanes' 16 bytes are neighbours
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
-                                 __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
-        } else {
-          uint4* dst = reinterpret_cast<uint4*>(a.out + token * a.o_tok + head * a.o_head + 32 * c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              w[k] = Elem<T>::pack(__uint_as_float(o[8 * e + 2 * k]) * inv,
-                                   __uint_as_float(o[8 * e + 2 * k + 1]) * inv);
-            dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+            part[(8 * c + e) * 256] =
+                make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                            __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+          continue;
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[k] = Elem<T>::pack(__uint_as_float(o[8 * e + 2 * k]) * inv,
+                                 __uint_as_float(o[8 * e + 2 * k + 1]) * inv);
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c & 1) * 4 + e) ^ (lane & 7)) << 4)) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if ((c & 1) == 0) continue;
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int r = 4 * k + (lane >> 3);
+          const int64_t at = __shfl_sync(0xffffffffu, dst, r);
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+          if (at >= 0) *reinterpret_cast<uint4*>(a.out + at + 32 * (c - 1) + 8 * (lane & 7)) = v;
+        }
+        __syncwarp();
       }
       if (live) {
-        if (splits > 1) a.part_ml[at] = make_float2(m, l);
-        else if (a.lse) a.lse[token * a.q_heads + head] = lse_of(m, l);
+        if (!whole)
+          a.part_ml[(2ll * blockIdx.x + (u.starts ? 1 : 0)) * 256 + t * kRows + row] = make_float2(m, l);
+        else if (a.lse)
+          a.lse[static_cast<int64_t>(u.token + local) * a.q_heads + head] = lse_of(m, l);
       }
       sm100::tc_fence_before();  // O is read before the next unit's first product
     }
@@ -545,40 +831,59 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
   }
 }
 
-// Joins the splits: D / 4 threads per (token, head).
+// Joins the cut units: CTA (c, y) takes 32 rows of the one that starts in
+// range c; its other pieces are the first ones of the ranges behind.
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) paged_prefill_join_kernel(PrefillArgs a, int grid) {
-  constexpr int kVec = D / 4;
-  int splits;
-  plan(a, grid, splits);
-  const int last = max(0, min(a.cu_q[a.pool.batch], a.n_tokens));
-  const int first = max(0, min(a.cu_q[0], a.n_tokens));
+  constexpr int kWarps = kJoinThreads / 32;
+  __shared__ uint2 s_out[32][D / 4 + 1];
   pdl_wait();
-  if (splits <= 1) return;
-  const int64_t rows = static_cast<int64_t>(a.n_tokens) * a.q_heads;
-  const int64_t r = blockIdx.x * static_cast<int64_t>(kJoinThreads / kVec) + threadIdx.x / kVec;
-  const int v = threadIdx.x % kVec;
-  if (r >= static_cast<int64_t>(last) * a.q_heads || r < static_cast<int64_t>(first) * a.q_heads)
-    return;
-  float m = -INFINITY;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, a.part_ml[s * rows + r].x);
-  const float base = m == -INFINITY ? 0.f : m;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
-    const float2 ml = a.part_ml[s * rows + r];
-    const float4 x = *reinterpret_cast<const float4*>(a.part_o + (s * rows + r) * D + 4 * v);
-    const float f = fast_exp2(ml.x - base);
-    l = fmaf(ml.y, f, l);
-    o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y);
-    o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
+  const CutUnit u = a.cuts[blockIdx.x];
+  if (u.slot < 0) return;
+  int end = blockIdx.x + 1;  // pieces in ranges [blockIdx.x, end)
+  while (end < grid) {
+    const CutUnit n = a.cuts[end];
+    if (!n.continues) break;
+    ++end;
+    if (n.ends) break;
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  const int64_t token = r / a.q_heads, head = r % a.q_heads;
-  *reinterpret_cast<uint2*>(a.out + token * a.o_tok + head * a.o_head + 4 * v) =
-      make_uint2(Elem<T>::pack(o.x * inv, o.y * inv), Elem<T>::pack(o.z * inv, o.w * inv));
-  if (a.lse && v == 0) a.lse[r] = lse_of(m, l);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row0 = blockIdx.y * kJoinRows, r = row0 + lane;
+  const int tok = r / kRows * a.tile_tokens + r % kRows / a.group;
+  const bool live = r % kRows / a.group < a.tile_tokens && tok < u.count;
+  auto slot = [&](int c) -> int64_t { return 2ll * c + (c == blockIdx.x ? 1 : 0); };
+  float m = -INFINITY, l = 0.f;
+  if (live) {
+    for (int c = blockIdx.x; c < end; ++c) m = fmaxf(m, a.part_ml[slot(c) * 256 + r].x);
+    const float base = m == -INFINITY ? 0.f : m;
+    for (int c = blockIdx.x; c < end; ++c) {
+      const float2 ml = a.part_ml[slot(c) * 256 + r];
+      l = fmaf(ml.y, fast_exp2(ml.x - base), l);
+    }
+    const float inv = inv_of(l);
+    for (int v = warp; v < D / 4; v += kWarps) {
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int c = blockIdx.x; c < end; ++c) {
+        const float f = fast_exp2(a.part_ml[slot(c) * 256 + r].x - base);
+        const float4 x = reinterpret_cast<const float4*>(a.part_o)[(slot(c) * (D / 4) + v) * 256 + r];
+        o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y);
+        o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
+      }
+      s_out[lane][v] = make_uint2(Elem<T>::pack(o.x * inv, o.y * inv), Elem<T>::pack(o.z * inv, o.w * inv));
+    }
+    if (warp == 0 && a.lse)
+      a.lse[static_cast<int64_t>(u.token + tok) * a.q_heads + u.kvh * a.group + r % kRows % a.group] =
+          lse_of(m, l);
+  }
+  __syncthreads();
+  for (int i = warp; i < kJoinRows; i += kWarps) {
+    const int q = row0 + i, t = q / kRows * a.tile_tokens + q % kRows / a.group;
+    if (q % kRows / a.group >= a.tile_tokens || t >= u.count) continue;
+    uint16_t* dst = a.out + static_cast<int64_t>(u.token + t) * a.o_tok +
+                    (u.kvh * a.group + q % kRows % a.group) * a.o_head;
+    if (lane < D / 4) reinterpret_cast<uint2*>(dst)[lane] = s_out[i][lane];
+  }
 }
 
 // 16-bit tensor of `rank` dimensions (innermost first, contiguous), boxes of
@@ -600,19 +905,16 @@ bool make_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Splits of a key axis that can fill the GPU: every sequence has at most
-// ceil(tokens / unit) units, so there are at least ceil(N / unit) of them.
-int most_splits(int n_tokens, int kv_heads, int tile_tokens, int table_width, int page_size) {
-  const int64_t units =
-      ceil_div(n_tokens, 2 * tile_tokens) * static_cast<int64_t>(kv_heads);
-  const int64_t blocks = ceil_div(static_cast<int64_t>(table_width) * page_size, kRows);
-  return static_cast<int>(std::max<int64_t>(1, std::min(num_sms() / units, blocks)));
+// Whether units may be cut: not where a sequence has few key blocks.
+bool may_cut(int table_width, int page_size) {
+  return ceil_div(static_cast<int64_t>(table_width) * page_size, kRows) > kWholeBlocks;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kCap, bool kBias>
 int32_t launch(const llmyb_paged_args* x, const PrefillArgs& a, cudaStream_t s) {
   using L = Layout<D>;
-  int32_t st = ensure_smem(paged_prefill_kernel<T, D>, L::kSmem);
+  auto* const kernel = paged_prefill_kernel<T, D, kCap, kBias>;
+  int32_t st = ensure_smem(kernel, L::kSmem);
   if (st) return st;
   CUtensorMap mq, mk, mv;
   {
@@ -632,15 +934,23 @@ int32_t launch(const llmyb_paged_args* x, const PrefillArgs& a, cudaStream_t s) 
       return LLMYB_EUNSUPPORTED;
   }
   const int grid = num_sms();
-  paged_prefill_kernel<T, D><<<grid, kThreads, L::kSmem, s>>>(mq, mk, mv, a);
+  kernel<<<grid, kThreads, L::kSmem, s>>>(mq, mk, mv, a);
   count_launch();
   st = launch_status();
-  if (st || a.max_splits <= 1) return st;
-  const int64_t ctas = ceil_div(static_cast<int64_t>(a.n_tokens) * a.q_heads, kJoinThreads / (D / 4));
-  cudaError_t e = launch_pdl(paged_prefill_join_kernel<T, D>, dim3(static_cast<unsigned>(ctas)),
-                             dim3(kJoinThreads), 0, s, a, grid);
+  if (st || !a.cut) return st;
+  const cudaError_t e = launch_pdl(paged_prefill_join_kernel<T, D>, dim3(grid, 256 / kJoinRows),
+                                   dim3(kJoinThreads), 0, s, a, grid);
   count_launch();
   return e == cudaSuccess ? launch_status() : static_cast<int32_t>(e);
+}
+
+// The score transforms are compiled in or out: their code between the loads
+// and the exponentials costs every block instruction fetches.
+template <typename T, int D>
+int32_t launch(const llmyb_paged_args* x, const PrefillArgs& a, cudaStream_t s) {
+  if (a.softcap > 0.f)
+    return a.slopes ? launch<T, D, true, true>(x, a, s) : launch<T, D, true, false>(x, a, s);
+  return a.slopes ? launch<T, D, false, true>(x, a, s) : launch<T, D, false, false>(x, a, s);
 }
 
 }  // namespace
@@ -648,17 +958,14 @@ int32_t launch(const llmyb_paged_args* x, const PrefillArgs& a, cudaStream_t s) 
 
 using namespace llmyb;
 
-LLMYB_API int64_t llmyb_paged_prefill_scratch_bytes(int32_t n_tokens, int32_t q_heads,
-                                                    int32_t kv_heads, int32_t head_dim,
-                                                    int32_t table_width, int32_t page_size) {
-  if (n_tokens < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0 ||
+LLMYB_API int64_t llmyb_paged_prefill_scratch_bytes(int32_t q_heads, int32_t kv_heads,
+                                                    int32_t head_dim, int32_t table_width,
+                                                    int32_t page_size) {
+  if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0 ||
       q_heads / kv_heads > kRows || table_width < 0 || page_size <= 0)
     return -1;
-  if (n_tokens == 0) return 0;
-  const int tile_tokens = kRows / (q_heads / kv_heads);
-  const int64_t splits = most_splits(n_tokens, kv_heads, tile_tokens, table_width, page_size);
-  if (splits <= 1) return 0;
-  return splits * n_tokens * q_heads * (head_dim + 2) * 4;
+  if (!may_cut(table_width, page_size)) return 0;
+  return static_cast<int64_t>(num_sms()) * (2 * 256 * (head_dim + 2) * 4 + sizeof(CutUnit));
 }
 
 LLMYB_API int32_t llmyb_paged_prefill(const llmyb_paged_args* x, void* stream) {
@@ -676,14 +983,15 @@ LLMYB_API int32_t llmyb_paged_prefill(const llmyb_paged_args* x, void* stream) {
   a.cu_q = x->cu_q, a.prefix = x->prefix, a.n_tokens = x->n_tokens, a.q_heads = x->q_heads;
   a.group = group, a.tile_tokens = kRows / group;
   a.window = x->window, a.scale = x->scale, a.softcap = x->softcap, a.slopes = x->slopes;
-  a.max_splits = most_splits(x->n_tokens, x->kv_heads, a.tile_tokens, x->table_width, x->page_size);
-  if (a.max_splits > 1 && !x->scratch) return LLMYB_EINVAL;
+  a.cut = may_cut(x->table_width, x->page_size);
+  if (a.cut && !x->scratch) return LLMYB_EINVAL;
   a.out = static_cast<uint16_t*>(x->out);
   a.o_tok = x->out_token_stride, a.o_head = x->out_head_stride;
   a.lse = x->lse;
+  const int64_t slots = 2ll * num_sms();
   a.part_o = static_cast<float*>(x->scratch);
-  a.part_ml = reinterpret_cast<float2*>(
-      a.part_o + static_cast<int64_t>(a.max_splits) * x->n_tokens * x->q_heads * x->head_dim);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * 256 * x->head_dim);
+  a.cuts = reinterpret_cast<CutUnit*>(a.part_ml + slots * 256);
   a.dev_status = x->dev_status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (x->fp16) return x->head_dim == 64 ? launch<__half, 64>(x, a, s) : launch<__half, 128>(x, a, s);

@@ -1268,7 +1268,7 @@ def _paged_call(entry: str, q, k_pages, v_pages, block_table, lengths, out, *, k
         if cu_q is None:
             need = lib.llmyb_paged_decode_scratch_bytes(heads, kv_heads, dim)
         else:
-            need = lib.llmyb_paged_prefill_scratch_bytes(n, heads, kv_heads, dim, width, page_size)
+            need = lib.llmyb_paged_prefill_scratch_bytes(heads, kv_heads, dim, width, page_size)
         if need > 0:
             scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
     f32 = torch.float32

@@ -853,9 +853,8 @@ int32_t llmyb_paged_decode(const llmyb_paged_args* args, void* stream);
  * j < prefix[b].  Rows that see no key give zeros.  Values of visible 128-key
  * blocks must be finite (rows outside the sequence may hold anything).
  * q_heads / kv_heads <= 128; scratch may be null where scratch_bytes is 0. */
-int64_t llmyb_paged_prefill_scratch_bytes(int32_t n_tokens, int32_t q_heads, int32_t kv_heads,
-                                          int32_t head_dim, int32_t table_width,
-                                          int32_t page_size);
+int64_t llmyb_paged_prefill_scratch_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                          int32_t table_width, int32_t page_size);
 int32_t llmyb_paged_prefill(const llmyb_paged_args* args, void* stream);
 
 #ifdef __cplusplus

@@ -168,13 +168,70 @@ struct Start {
   int b, piece, kvh;
 };
 
-// Before the roles part: every warp weighs some of the chunks into shared
-// memory, one warp looks the range's first unit up.  `sums` holds kSums chunk
-// sums; where a batch has more chunks (over 16,000 pieces), several share one.
+// Chunk sums of a batch of more than one chunk; where it has more chunks than
+// that (over 16,000 pieces), several share a sum.
 constexpr int kSums = 512;
 
+// numerator / denominator for values that mostly fit 32 bits
+__device__ __forceinline__ int64_t divide(int64_t n, int64_t d) {
+  if (((n | d) >> 32) == 0) return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
+  return n / d;
+}
+
+// This CTA's range of `total` positions.
+__device__ __forceinline__ void set_range(const PrefillArgs& a, int64_t total, Start& r) {
+  // as many ranges as can have kMinRange positions (1 where units are not
+  // cut); the CTAs behind have none
+  const int64_t most = max(static_cast<int64_t>(1), a.cut ? divide(total, kMinRange) : total);
+  const int64_t ranges = min(static_cast<int64_t>(gridDim.x), most);
+  const int64_t c = min(static_cast<int64_t>(blockIdx.x), ranges);
+  r.begin = divide(total * c, ranges);
+  r.end = divide(total * min(c + 1, ranges), ranges);
+}
+
+// If position r.begin lies in this chunk (`before` positions come before it):
+// the unit there.
+__device__ __forceinline__ bool find_unit(const PrefillArgs& a, int w, int b, int piece,
+                                          int64_t& before, Start& r) {
+  const int lane = threadIdx.x & 31;
+  int sum = w;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += y;
+  }
+  const uint32_t hit = __ballot_sync(0xffffffffu, before + sum > r.begin);
+  if (hit == 0) {
+    before += __shfl_sync(0xffffffffu, sum, 31);
+    return false;
+  }
+  const int h = __ffs(hit) - 1;
+  r.b = __shfl_sync(0xffffffffu, b, h);
+  r.piece = __shfl_sync(0xffffffffu, piece, h);
+  const int unit = __shfl_sync(0xffffffffu, w, h) / a.pool.kv_heads;
+  before += __shfl_sync(0xffffffffu, sum - w, h);
+  r.kvh = static_cast<int>(r.begin - before) / unit;
+  r.at = before + static_cast<int64_t>(r.kvh) * unit;
+  return true;
+}
+
+// Before the roles part, by the whole CTA; the result is warp 0's.  Beyond one
+// chunk every warp weighs some of them into shared memory (`sums`), and warp 0
+// looks the range's first unit up.
 __device__ __forceinline__ Start find_start(const PrefillArgs& a, int64_t* sums, int warps) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Start r = {0, 0, 0, a.pool.batch, 0, 0};
+  Group g;
+  g.load(a, 0);
+  if (a.pool.batch <= 32 && g.total <= 32) {
+    if (warp != 0) return r;
+    int b, piece;
+    const int w = g.weight(a, 0, b, piece);
+    set_range(a, __reduce_add_sync(0xffffffffu, w), r);
+    int64_t before = 0;
+    if (r.begin < r.end) find_unit(a, w, b, piece, before, r);
+    return r;
+  }
   // chunks at most: one per 32 pieces and one per group; pieces at most: one
   // per unit's tokens and one per sequence
   const int64_t pieces = a.n_tokens / (2 * a.tile_tokens) + a.pool.batch;
@@ -182,20 +239,19 @@ __device__ __forceinline__ Start find_start(const PrefillArgs& a, int64_t* sums,
   const int per = (most + kSums - 1) / kSums;
   for (int i = threadIdx.x; i < kSums; i += blockDim.x) sums[i] = 0;
   __syncthreads();
-  Group g;
   int chunk = 0;
   for (int b0 = 0; b0 < a.pool.batch; b0 += 32) {
-    g.load(a, b0);
+    if (b0 > 0) g.load(a, b0);
     for (int p0 = 0; p0 < g.total; p0 += 32, ++chunk) {
       if (chunk % warps != warp) continue;
-      int b, piece, w = g.weight(a, p0, b, piece);
-      w = __reduce_add_sync(0xffffffffu, w);
-      if (lane == 0) atomicAdd(reinterpret_cast<unsigned long long*>(&sums[min(chunk / per, kSums - 1)]),
+      int b, piece;
+      const int w = __reduce_add_sync(0xffffffffu, g.weight(a, p0, b, piece));
+      if (lane == 0)
+        atomicAdd(reinterpret_cast<unsigned long long*>(&sums[min(chunk / per, kSums - 1)]),
                   static_cast<unsigned long long>(w));
     }
   }
   __syncthreads();
-  Start r = {0, 0, 0, a.pool.batch, 0, 0};
   if (warp != 0) return r;
   int64_t mine = 0;  // of kSums / 32 neighbours
 #pragma unroll
@@ -206,14 +262,7 @@ __device__ __forceinline__ Start find_start(const PrefillArgs& a, int64_t* sums,
     const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += y;
   }
-  const int64_t total = __shfl_sync(0xffffffffu, inc, 31);
-  // as many ranges as can have kMinRange positions (1 where units are not
-  // cut); the CTAs behind have none
-  const int64_t most_ranges = max(static_cast<int64_t>(1), a.cut ? total / kMinRange : total);
-  const int64_t ranges = min(static_cast<int64_t>(gridDim.x), most_ranges);
-  const int64_t c = min(static_cast<int64_t>(blockIdx.x), ranges);
-  r.begin = total * c / ranges;
-  r.end = total * min(c + 1, ranges) / ranges;
+  set_range(a, __shfl_sync(0xffffffffu, inc, 31), r);
   if (r.begin >= r.end) return r;
   // the sum, then the chunk, then the piece that holds r.begin
   const int l = __ffs(__ballot_sync(0xffffffffu, inc > r.begin)) - 1;
@@ -222,31 +271,12 @@ __device__ __forceinline__ Start find_start(const PrefillArgs& a, int64_t* sums,
   while (before + sums[at] <= r.begin) before += sums[at++];
   chunk = 0;
   for (int b0 = 0; b0 < a.pool.batch; b0 += 32) {
-    g.load(a, b0);
+    if (a.pool.batch > 32) g.load(a, b0);
     const int chunks = (g.total + 31) / 32;
-    if (chunk + chunks > at * per) {
-      for (int k = max(0, at * per - chunk); k < chunks; ++k) {
-        int b, piece;
-        const int w = g.weight(a, 32 * k, b, piece);
-        int sum = w;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, sum, o);
-          if (lane >= o) sum += y;
-        }
-        const uint32_t hit = __ballot_sync(0xffffffffu, before + sum > r.begin);
-        if (hit != 0) {
-          const int h = __ffs(hit) - 1;
-          r.b = __shfl_sync(0xffffffffu, b, h);
-          r.piece = __shfl_sync(0xffffffffu, piece, h);
-          const int unit = __shfl_sync(0xffffffffu, w, h) / a.pool.kv_heads;
-          before += __shfl_sync(0xffffffffu, sum - w, h);
-          r.kvh = static_cast<int>((r.begin - before) / unit);
-          r.at = before + static_cast<int64_t>(r.kvh) * unit;
-          return r;
-        }
-        before += __shfl_sync(0xffffffffu, sum, 31);
-      }
+    for (int k = max(0, at * per - chunk); k < chunks; ++k) {
+      int b, piece;
+      const int w = g.weight(a, 32 * k, b, piece);
+      if (find_unit(a, w, b, piece, before, r)) return r;
     }
     chunk += chunks;
   }
@@ -840,22 +870,28 @@ __global__ void __launch_bounds__(kJoinThreads) paged_prefill_join_kernel(Prefil
   pdl_wait();
   const CutUnit u = a.cuts[blockIdx.x];
   if (u.slot < 0) return;
-  int end = blockIdx.x + 1;  // pieces in ranges [blockIdx.x, end)
-  while (end < grid) {
-    const CutUnit n = a.cuts[end];
-    if (!n.continues) break;
-    ++end;
-    if (n.ends) break;
-  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // its pieces lie in ranges [blockIdx.x, end)
+  int end = blockIdx.x + 1;
+  for (bool more = true; more; ) {
+    const int c = end + lane;
+    CutUnit n = {0, 0, 0, 0, 0, 0};
+    if (c < grid) n = a.cuts[c];
+    const uint32_t stop = __ballot_sync(0xffffffffu, !n.continues || n.ends);
+    const int last = __ffs(stop) - 1;  // -1: all 32 go on
+    more = stop == 0;
+    end += more ? 32 : last + (__shfl_sync(0xffffffffu, n.continues, max(last, 0)) ? 1 : 0);
+  }
   const int row0 = blockIdx.y * kJoinRows, r = row0 + lane;
   const int tok = r / kRows * a.tile_tokens + r % kRows / a.group;
   const bool live = r % kRows / a.group < a.tile_tokens && tok < u.count;
   auto slot = [&](int c) -> int64_t { return 2ll * c + (c == blockIdx.x ? 1 : 0); };
   float m = -INFINITY, l = 0.f;
   if (live) {
+#pragma unroll 4
     for (int c = blockIdx.x; c < end; ++c) m = fmaxf(m, a.part_ml[slot(c) * 256 + r].x);
     const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
     for (int c = blockIdx.x; c < end; ++c) {
       const float2 ml = a.part_ml[slot(c) * 256 + r];
       l = fmaf(ml.y, fast_exp2(ml.x - base), l);

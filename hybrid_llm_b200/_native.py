@@ -7,11 +7,13 @@ call raises, so a GPU run can never silently take a CPU or eager path.
 from __future__ import annotations
 
 import ctypes as C
-import struct
+import importlib.machinery
+import importlib.util
 import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libllmyb.so"
+TORCH_LIB_PATH = LIB_PATH.with_name("llmyb_torch.so")
 
 LLMYB_OK = 0
 LLMYB_EINVAL = 1
@@ -128,20 +130,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "llmyb_router_ctx_prefill": (I32, [P, I32, I32, I32, I32, P, P, P, P, P]),
     "llmyb_router_ctx_step": (I32, [P, I32, I32, I32, P, P, P, P, P, P]),
     # paged key-value cache
-    "llmyb_paged_append": (I32, [C.c_char_p, P]),
+    "llmyb_paged_append": (I32, [P, P]),
     "llmyb_paged_decode_scratch_bytes": (I64, [I32, I32, I32]),
-    "llmyb_paged_decode": (I32, [C.c_char_p, P]),
+    "llmyb_paged_decode": (I32, [P, P]),
     "llmyb_paged_prefill_scratch_bytes": (I64, [I32, I32, I32, I32, I32]),
-    "llmyb_paged_prefill": (I32, [C.c_char_p, P]),
+    "llmyb_paged_prefill": (I32, [P, P]),
 }
-
-# llmyb_paged_args of include/llmyb.h: 17 pointers, 12 strides, 12 int32, 3
-# floats, 1 int32.  A packed block costs a tenth of ctypes' conversion of as
-# many arguments, which would be most of a one-token call.
-PAGED_ARGS = struct.Struct("=17Q12q12i3fi")
 
 _lock = threading.Lock()
 _lib: C.CDLL | None = None
+_torch_module = None
 
 
 def lib() -> C.CDLL:
@@ -162,6 +160,25 @@ def lib() -> C.CDLL:
                 fn.argtypes = args
             _lib = handle
     return _lib
+
+
+def torch_module():
+    """The tensor-level module (csrc/torch), loaded once; raise if it is absent."""
+    global _torch_module
+    if _torch_module is None:
+        lib()
+        with _lock:
+            if _torch_module is None:
+                if not TORCH_LIB_PATH.exists():
+                    raise RuntimeError(f"llmyb torch module not found at {TORCH_LIB_PATH}; "
+                                       "build it with `python -m hybrid_llm_b200.build`")
+                import torch  # noqa: F401  (its libraries resolve the module's symbols)
+                loader = importlib.machinery.ExtensionFileLoader("llmyb_torch", str(TORCH_LIB_PATH))
+                spec = importlib.util.spec_from_loader("llmyb_torch", loader)
+                module = importlib.util.module_from_spec(spec)
+                loader.exec_module(module)
+                _torch_module = module
+    return _torch_module
 
 
 def check(status: int, what: str) -> None:

@@ -3,20 +3,25 @@
 ``python -m hybrid_llm_b200.build`` compiles every ``csrc/*.cu`` file with
 nvcc for ``sm_100a`` and links ``hybrid_llm_b200/lib/libllmyb.so``.  Objects
 are cached under ``_build/`` and rebuilt only when a source or header is newer.
+``csrc/torch/*.cpp`` becomes ``hybrid_llm_b200/lib/llmyb_torch.so``, a Python
+module that takes torch tensors and calls the library (g++, torch's headers).
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB_DIR = PKG / "lib"
 LIB = LIB_DIR / "libllmyb.so"
+TORCH_LIB = LIB_DIR / "llmyb_torch.so"
 BUILD = PKG.parent / "_build"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -49,6 +54,25 @@ def _compile(src: Path, obj: Path, verbose: bool) -> None:
         print(res.stdout + res.stderr, file=sys.stderr)
 
 
+def _torch_module(verbose: bool) -> None:
+    """The tensor-level module; torch itself is not imported."""
+    torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    cuda = Path(nvcc()).resolve().parents[1]
+    tmp = TORCH_LIB.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-I{sysconfig.get_paths()['include']}", f"-isystem{torch / 'include'}",
+           f"-isystem{torch / 'include/torch/csrc/api/include'}", f"-isystem{cuda / 'include'}",
+           *map(str, sorted((CSRC / "torch").glob("*.cpp"))), "-o", str(tmp),
+           f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           f"-L{LIB_DIR}", "-lllmyb", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on csrc/torch:\n{res.stdout}\n{res.stderr}")
+    if verbose and (res.stdout or res.stderr):
+        print(res.stdout + res.stderr, file=sys.stderr)
+    os.replace(tmp, TORCH_LIB)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile and link; returns the path of the shared library."""
     BUILD.mkdir(exist_ok=True)
@@ -74,6 +98,10 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
+    made = TORCH_LIB.stat().st_mtime if TORCH_LIB.exists() and not force else 0.0
+    inputs = [*(CSRC / "torch").glob("*.cpp"), *(PKG.parent / "include").glob("*.h")]
+    if made < max(f.stat().st_mtime for f in inputs):
+        _torch_module(verbose)
     return LIB
 
 

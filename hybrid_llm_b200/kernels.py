@@ -1175,116 +1175,23 @@ def csa_remote_step(x: torch.Tensor, q: torch.Tensor, w_comp: torch.Tensor, rati
 
 
 # ------------------------------------------------------ paged key-value cache
-# These checks are most of a one-token call's host time: each attribute of a
-# tensor is asked for once.
-PAGE_SIZES = (16, 32, 64, 128, 256)
+# The checks, the allocations and the calls are in csrc/torch/paged.cpp: in
+# Python they took longer than a one-token call on the GPU.
+_APPEND, _DECODE, _PREFILL = range(3)
 
 
-def _paged_rows(t: torch.Tensor, name: str, heads: int | None, dim: int, dtype: torch.dtype,
-                tokens: int | None = None):
-    """(pointer, token stride, head stride) of [tokens, heads, dim] rows."""
-    shape, (sn, sh, sd), p = t.shape, t.stride(), t.data_ptr()
-    if t.dtype is not dtype or shape[2] != dim or (heads is not None and shape[1] != heads) or (
-            tokens is not None and shape[0] != tokens):
-        raise ValueError(f"{name} must be [{tokens or 'tokens'}, {heads or 'heads'}, {dim}] {dtype}")
-    if sd != 1 or (sn | sh) & 7 or p & 15:
-        raise ValueError(f"{name}: contiguous head dimension, 16-byte aligned rows and heads")
-    return p, sn, sh
+def _paged_status(q: torch.Tensor) -> torch.Tensor:
+    index = q.get_device()
+    if index < 0:
+        raise RuntimeError("llmyb kernels take CUDA tensors only (no CPU fallback)")
+    status = _status.get(index)
+    return device_status(q.device) if status is None else status
 
 
-def _paged_vector(t: torch.Tensor | None, name: str, dtype: torch.dtype, n: int) -> int:
-    if t is None:
-        return 0
-    if t.dtype is not dtype or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name} must be contiguous {dtype} [{n}]")
-    return t.data_ptr()
-
-
-def _paged_call(entry: str, q, k_pages, v_pages, block_table, lengths, out, *, k=None, v=None,
-                cu_q=None, prefix=None, slopes=None, q_norm=None, k_norm=None, inv_freq=None,
-                lse=None, window=0, interleaved=False, scale=1.0, softcap=0.0, eps=0.0):
-    """Checks the arguments, allocates the output and the scratch, makes the call."""
-    dev = q.get_device()
-    for t in (k_pages, v_pages, block_table, lengths, out, k, v, cu_q, prefix, slopes, q_norm,
-              k_norm, inv_freq, lse):
-        if t is not None and t.get_device() != dev:
-            dev = -1
-    if dev < 0:
-        raise RuntimeError("llmyb kernels take CUDA tensors only (no CPU fallback), all on one "
-                           "device")
-    if dev != torch.cuda.current_device():
-        raise ValueError("paged cache tensors must be on the current CUDA device")
-    dtype, shape, strides = k_pages.dtype, k_pages.shape, k_pages.stride()
-    if (len(shape) != 4 or (dtype is not torch.bfloat16 and dtype is not torch.float16)
-            or v_pages.dtype is not dtype or v_pages.shape != shape
-            or v_pages.stride() != strides):
-        raise ValueError("k_pages and v_pages must be alike: [pages, kv_heads, page_size, head_dim] "
-                         "bf16 or fp16 with the same strides")
-    pages, kv_heads, page_size, dim = shape
-    sp, sh, sr, sd = strides
-    kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
-    if page_size not in PAGE_SIZES or (dim != 64 and dim != 128):
-        raise ValueError(f"pages of {PAGE_SIZES} rows and head dimensions 64 or 128 are served")
-    if sd != 1 or (sp | sh | sr) & 7 or (kp | vp) & 15:
-        raise ValueError("pages: contiguous head dimension, 16-byte aligned pages, heads and rows")
-    batch, width = block_table.shape
-    st, sc = block_table.stride()
-    if block_table.dtype is not torch.int32 or (sc != 1 and width > 1):
-        raise ValueError("block_table must be int32 [batch, pages per sequence]")
-    lp = _paged_vector(lengths, "lengths", torch.int32, batch)
-    if q.dim() != 3:
-        raise ValueError("q must be [tokens, heads, head_dim]")
-    n, heads, _ = q.shape
-    qp, qn, qh = _paged_rows(q, "q", None, dim, dtype)
-    kr = vr = (0, 0, 0)
-    half = 0
-    if k is not None:
-        kr = _paged_rows(k, "k", kv_heads, dim, dtype, n)
-        vr = _paged_rows(v, "v", kv_heads, dim, dtype, n)
-        half = 0 if inv_freq is None else inv_freq.numel()
-        if half & 7 or 2 * half > dim:
-            raise ValueError(f"inv_freq must have a multiple of 8 values, at most {dim // 2}")
-    else:
-        if kv_heads < 1 or heads % kv_heads:
-            raise ValueError("query heads must be a multiple of the kv heads")
-        if not softcap >= 0.0 or window < 0:
-            raise ValueError("softcap and window must be >= 0 (0: none)")
-        scale = dim ** -0.5 if scale is None else float(scale)
-        if not scale > 0.0:
-            raise ValueError("scale must be positive")
-        if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (n, heads)
-                                or not lse.is_contiguous()):
-            raise ValueError("lse must be contiguous fp32 [tokens, heads]")
-    if cu_q is None and n != batch:
-        raise ValueError("without cu_q there is one token per sequence of block_table")
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        op, on, oh = out.data_ptr(), heads * dim, dim
-    else:
-        op, on, oh = _paged_rows(out, "out", heads, dim, dtype, n)
-    lib = _native.lib()
-    scratch = None
-    if k is None:
-        if cu_q is None:
-            need = lib.llmyb_paged_decode_scratch_bytes(heads, kv_heads, dim)
-        else:
-            need = lib.llmyb_paged_prefill_scratch_bytes(heads, kv_heads, dim, width, page_size)
-        if need > 0:
-            scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-    f32 = torch.float32
-    args = _native.PAGED_ARGS.pack(
-        qp, kr[0], vr[0], _paged_vector(q_norm, "q_norm", f32, dim),
-        _paged_vector(k_norm, "k_norm", f32, dim), _paged_vector(inv_freq, "inv_freq", f32, half),
-        kp, vp, block_table.data_ptr(), lp, _paged_vector(cu_q, "cu_q", torch.int32, batch + 1),
-        _paged_vector(prefix, "prefix", torch.int32, batch),
-        _paged_vector(slopes, "slopes", f32, heads), op, 0 if lse is None else lse.data_ptr(),
-        0 if scratch is None else scratch.data_ptr(), device_status(q.device).data_ptr(), qn, qh,
-        kr[1], kr[2], vr[1], vr[2], on, oh, sp, sh, sr, st, n, batch, heads, kv_heads, dim,
-        dtype is torch.float16, pages, page_size, width, window, half, interleaved, scale, softcap,
-        eps, 0)
-    status = getattr(lib, entry)(args, torch._C._cuda_getCurrentRawStream(dev))
-    if status:
-        _native.check(status, entry)
+def _paged_call(kind: int, q, *args) -> torch.Tensor:
+    out = _native.torch_module().call(kind, q, *args)
+    if type(out) is tuple:
+        _native.check(*out)
     return out
 
 
@@ -1306,9 +1213,9 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     sequence) are the last positions of sequence b.  Rows behind cu_q[B] are
     left alone; a token at a negative position (a slot of length 0) is not
     stored and its query is zero.  q_out may be q."""
-    return _paged_call("llmyb_paged_append", q, k_pages, v_pages, block_table, lengths, q_out, k=k,
-                       v=v, cu_q=cu_q, inv_freq=inv_freq, interleaved=interleaved, q_norm=q_norm,
-                       k_norm=k_norm, eps=eps)
+    return _paged_call(_APPEND, q, k, v, k_pages, v_pages, block_table, lengths, cu_q, None, None,
+                       q_norm, k_norm, inv_freq, q_out, None, _paged_status(q), None, 0.0,
+                       eps, 0, interleaved)
 
 
 def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -1323,8 +1230,9 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     at distance < window.  Query head h reads kv head h // (Hq / Hkv).  A
     sequence of length 0 gives zeros.  lse (fp32 [B, Hq]) receives the natural
     log-sum-exp of the scores."""
-    return _paged_call("llmyb_paged_decode", q, k_pages, v_pages, block_table, lengths, out,
-                       scale=scale, softcap=softcap, window=window, slopes=slopes, lse=lse)
+    return _paged_call(_DECODE, q, None, None, k_pages, v_pages, block_table, lengths, None, None,
+                       slopes, None, None, None, out, lse, _paged_status(q), scale, softcap,
+                       0.0, window, False)
 
 
 def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -1340,10 +1248,6 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     (window > 0) or, instead of a window, also those j < prefix[b] (int32 [B]:
     a bidirectional prefix).  Rows that see no key give zeros; rows behind
     cu_q[B] are left alone.  lse: fp32 [N, Hq]."""
-    if prefix is not None and window:
-        raise ValueError("a prefix and a window exclude each other")
-    if q.shape[1] > 128 * k_pages.shape[1]:
-        raise ValueError("at most 128 query heads per kv head")
-    return _paged_call("llmyb_paged_prefill", q, k_pages, v_pages, block_table, lengths, out,
-                       cu_q=cu_q, scale=scale, softcap=softcap, window=window, slopes=slopes,
-                       prefix=prefix, lse=lse)
+    return _paged_call(_PREFILL, q, None, None, k_pages, v_pages, block_table, lengths, cu_q,
+                       prefix, slopes, None, None, None, out, lse, _paged_status(q), scale,
+                       softcap, 0.0, window, False)

@@ -10,12 +10,18 @@
 // The angle is formed and reduced to [-pi, pi] in 64 bits (a product rounded
 // to 32 bits is off by 0.06 rad at position 10^6), its sine and cosine and
 // everything else in 32, with one rounding at the store.
+//
+// Bound by its bytes, or by latency for a few tokens.  A warp takes some heads
+// of one token, 16 bytes per lane: its rows are asked for first, and the
+// sequence's lookups and the angles (two per lane, handed round by shuffles, the
+// same for every head) run while they travel; no barrier, no shared memory.
 #include "paged.cuh"
+#include "tma_host.h"
 
 namespace llmyb {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // 8 warps that know nothing of each other
 
 struct AppendArgs {
   const uint16_t *q, *k, *v;
@@ -33,133 +39,190 @@ struct AppendArgs {
   int32_t* dev_status;
 };
 
-// One CTA per token; DH / 8 lanes per head, 16 bytes each.
-template <typename T, int DH>
-__global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a) {
-  constexpr int kLanes = DH / 8;
-  __shared__ float2 s_rot[DH / 2];  // (cos, sin) of the token's angles
-  const int tok = blockIdx.x, tid = threadIdx.x;
+// How a token's heads are dealt to warps: `rounds` rounds of 32 / (DH / 8) heads
+// each, every warp with heads of one kind (queries, keys or values).
+struct Parts {
+  int q, kv;  // warps for the queries, for the keys and for the values
+};
+
+template <typename T, int DH, int kRounds>
+__global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(AppendArgs a, Parts parts) {
+  constexpr int kLanes = DH / 8, kHeads = 32 / kLanes;
+  const int lane = threadIdx.x & 31, l = lane % kLanes;
+  const int64_t w = blockIdx.x * static_cast<int64_t>(kThreads / 32) + (threadIdx.x >> 5);
+  const int per = parts.q + 2 * parts.kv;
+  const int tok = static_cast<int>(w / per);
+  if (tok >= a.n_tokens) return;
+  int part = static_cast<int>(w % per);
+  const int kind = part < parts.q ? 0 : part < parts.q + parts.kv ? 1 : 2;
+  part -= kind == 0 ? 0 : kind == 1 ? parts.q : parts.q + parts.kv;
+  const int heads = kind == 0 ? a.q_heads : a.pool.kv_heads;
+  const int h0 = part * (kRounds * kHeads) + lane / kLanes;
+  const uint16_t* const src = (kind == 0   ? a.q + tok * a.q_tok
+                               : kind == 1 ? a.k + tok * a.k_tok
+                                           : a.v + tok * a.v_tok) + 8 * l;
+  const int64_t src_head = kind == 0 ? a.q_head : kind == 1 ? a.k_head : a.v_head;
+  uint4 raw[kRounds];
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const int h = h0 + i * kHeads;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (h < heads) raw[i] = __ldcs(reinterpret_cast<const uint4*>(src + h * src_head));
+  }
   int b = tok, pos;
   if (a.cu_q != nullptr) {
-    if (tok >= a.cu_q[a.pool.batch]) return;  // rows behind the last sequence
-    int lo = 0, hi = a.pool.batch;            // cu_q[lo] <= tok < cu_q[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu_q[mid] <= tok) lo = mid;
-      else hi = mid;
+    const int end = a.cu_q[a.pool.batch];
+    // the last b with cu_q[b] <= tok, 32 candidates at a time
+    b = 0;
+    for (int n = a.pool.batch; n > 1;) {
+      const int step = (n + 31) / 32, at = (lane + 1) * step;
+      const bool below = at < n && a.cu_q[b + at] <= tok;
+      const int skip = __popc(__ballot_sync(0xffffffffu, below)) * step;
+      b += skip;
+      n = min(step, n - skip);
     }
-    b = lo;
+    if (tok >= end) return;  // rows behind the last sequence
     pos = a.pool.lengths[b] - a.cu_q[b + 1] + tok;
   } else {
     pos = a.pool.lengths[b] - 1;
   }
-  if (tid < a.half) {
-    constexpr double kTwoPi = 6.283185307179586476925286766559;
-    const double t = static_cast<double>(pos) * static_cast<double>(a.inv_freq[tid]);
-    float s, c;
-    sincosf(static_cast<float>(t - rint(t * (1.0 / kTwoPi)) * kTwoPi), &s, &c);
-    s_rot[tid] = make_float2(c, s);
-  }
-  // the page of this position
-  const int page_i = pos >> a.pool.page_shift;
-  int page = -1;
-  if (pos >= 0) {
+  uint16_t* dst = a.q_out + tok * a.o_tok;
+  int64_t dst_head = a.o_head;
+  if (kind != 0) {
+    if (pos < 0) return;  // a slot without a token
+    const int page_i = pos >> a.pool.page_shift;
+    int page = -1;
     if (page_i < a.pool.table_width) page = a.pool.table[b * a.pool.table_stride + page_i];
     if (page < 0 || page >= a.pool.num_pages) {
-      page = -1;
-      if (tid == 0) report_status(a.dev_status, LLMYB_EINVAL);
+      if (lane == 0) report_status(a.dev_status, LLMYB_EINVAL);
+      return;
     }
+    dst = (kind == 1 ? a.k_pages : a.v_pages) + static_cast<int64_t>(page) * a.pool.page_stride +
+          (pos & ((1 << a.pool.page_shift) - 1)) * a.pool.row_stride;
+    dst_head = a.pool.head_stride;
   }
-  const int64_t in_page = static_cast<int64_t>(page) * a.pool.page_stride +
-                          (pos & ((1 << a.pool.page_shift) - 1)) * a.pool.row_stride;
-  __syncthreads();
+  dst += 8 * l;
+  const float* const norm = kind == 0 ? a.q_norm : a.k_norm;
+  const bool copy = kind == 2 || (norm == nullptr && a.half == 0);
 
-  const int l = tid % kLanes;
-  const int heads = a.q_heads + 2 * a.pool.kv_heads;
-  for (int h0 = tid / kLanes; h0 < (heads + kThreads / kLanes - 1) / (kThreads / kLanes) *
-                                       (kThreads / kLanes);
-       h0 += kThreads / kLanes) {
-    const bool live = h0 < heads;
-    const int h = min(h0, heads - 1);
-    const uint16_t* src;
-    uint16_t* dst;
-    const float* w = nullptr;
-    bool turn = false, store;
-    if (h < a.q_heads) {
-      src = a.q + tok * a.q_tok + h * a.q_head;
-      dst = a.q_out + tok * a.o_tok + h * a.o_head;
-      w = a.q_norm;
-      turn = true;
-      store = live;
-    } else if (h < a.q_heads + a.pool.kv_heads) {
-      const int g = h - a.q_heads;
-      src = a.k + tok * a.k_tok + g * a.k_head;
-      dst = a.k_pages + in_page + g * a.pool.head_stride;
-      w = a.k_norm;
-      turn = true;
-      store = live && page >= 0;
-    } else {
-      const int g = h - a.q_heads - a.pool.kv_heads;
-      src = a.v + tok * a.v_tok + g * a.v_head;
-      dst = a.v_pages + in_page + g * a.pool.head_stride;
-      store = live && page >= 0;
-    }
-    uint4 raw = *reinterpret_cast<const uint4*>(src + 8 * l);
-    if (pos < 0) raw = make_uint4(0, 0, 0, 0);  // a slot without a token: its query is zero
-    float x[8];
-    {
-      const float2 p0 = Elem<T>::unpack(raw.x), p1 = Elem<T>::unpack(raw.y),
-                   p2 = Elem<T>::unpack(raw.z), p3 = Elem<T>::unpack(raw.w);
-      x[0] = p0.x, x[1] = p0.y, x[2] = p1.x, x[3] = p1.y;
-      x[4] = p2.x, x[5] = p2.y, x[6] = p3.x, x[7] = p3.y;
-    }
-    // the shuffles run in every lane: lane groups of one warp may hold
-    // different kinds of heads
-    float ss = 0.f;
+  // x'_k = r (x_k u_k + y_k v_k), y the other member of the pair and r the
+  // inverse RMS: u = weight cos, v = -+ the other's weight sin, the same for
+  // every head of this warp
+  float u[8], v[8];
+  const int d = a.half / 8;  // lanes between the two members of a half-split pair
+  const bool second = l >= d && l < 2 * d;
+  const int other = l < d ? l + d : second ? l - d : l;
+  const bool turns = a.half > 0 && 8 * l < 2 * a.half;
+  if (!copy) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (w != nullptr) {
-      const float r = rsqrtf(ss * (1.f / DH) + a.eps);
-      const float4 w0 = *reinterpret_cast<const float4*>(w + 8 * l);
-      const float4 w1 = *reinterpret_cast<const float4*>(w + 8 * l + 4);
-      x[0] *= r * w0.x, x[1] *= r * w0.y, x[2] *= r * w0.z, x[3] *= r * w0.w;
-      x[4] *= r * w1.x, x[5] *= r * w1.y, x[6] *= r * w1.z, x[7] *= r * w1.w;
+    for (int k = 0; k < 8; ++k) {
+      u[k] = norm ? norm[8 * l + k] : 1.f;
+      v[k] = 0.f;
     }
     if (a.half > 0) {
-      if (a.interleaved) {
-        if (turn && 8 * l < 2 * a.half) {
+      float c[2] = {1.f, 1.f}, s[2] = {0.f, 0.f};  // of pairs 2 lane and 2 lane + 1
+      if (2 * lane < a.half) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 r = s_rot[4 * l + i];
-            const float u = x[2 * i], v = x[2 * i + 1];
-            x[2 * i] = u * r.x - v * r.y;
-            x[2 * i + 1] = v * r.x + u * r.y;
+        for (int i = 0; i < 2; ++i) {
+          constexpr double kTwoPi = 6.283185307179586476925286766559;
+          const double t = static_cast<double>(pos) * static_cast<double>(a.inv_freq[2 * lane + i]);
+          // 2^-21 of absolute error on [-pi, pi]
+          __sincosf(static_cast<float>(t - rint(t * (1.0 / kTwoPi)) * kTwoPi), &s[i], &c[i]);
+        }
+      }
+      if (a.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int from = (4 * l + i) >> 1 & 31;
+          const float cc = __shfl_sync(0xffffffffu, c[i & 1], from);
+          const float ss = __shfl_sync(0xffffffffu, s[i & 1], from);
+          if (turns) {
+            const float w0 = u[2 * i], w1 = u[2 * i + 1];
+            u[2 * i] = w0 * cc, v[2 * i] = -w1 * ss;
+            u[2 * i + 1] = w1 * cc, v[2 * i + 1] = w0 * ss;
           }
         }
       } else {
-        const int d = a.half / 8;  // lanes between the two members of a pair
-        const bool first = l < d, second = l >= d && l < 2 * d;
-        const int peer = (threadIdx.x & 31) + (first ? d : second ? -d : 0);
-        const int at = first ? 8 * l : second ? 8 * (l - d) : 0;
+        const int first = 8 * (second ? l - d : l);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float y = __shfl_sync(0xffffffffu, x[i], peer);
-          const float2 r = s_rot[at + i];
-          if (turn && first) x[i] = x[i] * r.x - y * r.y;
-          if (turn && second) x[i] = x[i] * r.x + y * r.y;
+        for (int k = 0; k < 8; ++k) {
+          const int from = (first + k) >> 1 & 31;
+          const float cc = __shfl_sync(0xffffffffu, c[k & 1], from);
+          const float ss = __shfl_sync(0xffffffffu, s[k & 1], from);
+          if (turns) {
+            v[k] = (second ? ss : -ss) * (norm ? norm[8 * other + k] : 1.f);
+            u[k] *= cc;
+          }
         }
       }
     }
-    if (store) {
-      uint4 o = raw;  // values pass unchanged
-      if (turn && (w != nullptr || a.half > 0))
-        o = make_uint4(Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]),
-                       Elem<T>::pack(x[4], x[5]), Elem<T>::pack(x[6], x[7]));
-      *reinterpret_cast<uint4*>(dst + 8 * l) = o;
-    }
   }
+  const int peer = lane - l + other;
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const int h = h0 + i * kHeads;
+    if (part * (kRounds * kHeads) + i * kHeads >= heads) break;
+    uint4 o = raw[i];
+    if (pos < 0) o = make_uint4(0, 0, 0, 0);  // its query is zero
+    if (!copy) {
+      uint4 p = o;  // the pairs' other members
+      if (!a.interleaved && a.half > 0) {
+        p.x = __shfl_sync(0xffffffffu, o.x, peer), p.y = __shfl_sync(0xffffffffu, o.y, peer);
+        p.z = __shfl_sync(0xffffffffu, o.z, peer), p.w = __shfl_sync(0xffffffffu, o.w, peer);
+      }
+      const float2 x[4] = {Elem<T>::unpack(o.x), Elem<T>::unpack(o.y), Elem<T>::unpack(o.z),
+                           Elem<T>::unpack(o.w)};
+      float r = 1.f;
+      if (norm != nullptr) {
+        float ss = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) ss = fmaf(x[k].x, x[k].x, fmaf(x[k].y, x[k].y, ss));
+#pragma unroll
+        for (int k = kLanes / 2; k > 0; k >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, k);
+        r = rsqrtf(ss * (1.f / DH) + a.eps);
+      }
+      float2 z[4];
+      if (!turns) {  // by itself: zero times an infinity is none
+#pragma unroll
+        for (int k = 0; k < 4; ++k) z[k] = make_float2(x[k].x * u[2 * k], x[k].y * u[2 * k + 1]);
+      } else if (a.interleaved) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          z[k] = make_float2(fmaf(x[k].x, u[2 * k], x[k].y * v[2 * k]),
+                             fmaf(x[k].y, u[2 * k + 1], x[k].x * v[2 * k + 1]));
+      } else {
+        const float2 y[4] = {Elem<T>::unpack(p.x), Elem<T>::unpack(p.y), Elem<T>::unpack(p.z),
+                             Elem<T>::unpack(p.w)};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          z[k] = make_float2(fmaf(x[k].x, u[2 * k], y[k].x * v[2 * k]),
+                             fmaf(x[k].y, u[2 * k + 1], y[k].y * v[2 * k + 1]));
+      }
+      o = make_uint4(Elem<T>::pack(z[0].x * r, z[0].y * r), Elem<T>::pack(z[1].x * r, z[1].y * r),
+                     Elem<T>::pack(z[2].x * r, z[2].y * r), Elem<T>::pack(z[3].x * r, z[3].y * r));
+    }
+    if (h < heads) *reinterpret_cast<uint4*>(dst + h * dst_head) = o;
+  }
+}
+
+// Rounds per warp: one where that many warps do not fill the GPU's 64 per SM
+// (a token's latency counts), else eight, so that a token's lookups and angles
+// serve several heads: 14117 tokens of 16 + 2 x 16 heads, 347 MB, take 77 us
+// (0.69 of the copy rate) with eight, 85 us with four; one CTA per token with
+// the angles in shared memory took 129 us.
+template <typename T, int DH, int kRounds>
+void launch(const AppendArgs& a, cudaStream_t s) {
+  constexpr int kHeads = kRounds * (256 / DH);
+  const Parts p = {(a.q_heads + kHeads - 1) / kHeads, (a.pool.kv_heads + kHeads - 1) / kHeads};
+  const int64_t warps = static_cast<int64_t>(a.n_tokens) * (p.q + 2 * p.kv);
+  paged_append_kernel<T, DH, kRounds>
+      <<<static_cast<unsigned>(ceil_div(warps, kThreads / 32)), kThreads, 0, s>>>(a, p);
+}
+template <typename T, int DH>
+void launch(const AppendArgs& a, cudaStream_t s) {
+  const int64_t rounds = ceil_div(a.q_heads + 2 * a.pool.kv_heads, 256 / DH);
+  if (a.n_tokens * rounds <= 64ll * num_sms()) launch<T, DH, 1>(a, s);
+  else launch<T, DH, 8>(a, s);
 }
 
 }  // namespace
@@ -194,13 +257,12 @@ LLMYB_API int32_t llmyb_paged_append(const llmyb_paged_args* x, void* stream) {
   a.inv_freq = x->inv_freq, a.half = x->rope_half, a.interleaved = x->interleaved;
   a.dev_status = x->dev_status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int n = x->n_tokens;
   if (x->fp16) {
-    if (x->head_dim == 64) paged_append_kernel<__half, 64><<<n, kThreads, 0, s>>>(a);
-    else paged_append_kernel<__half, 128><<<n, kThreads, 0, s>>>(a);
+    if (x->head_dim == 64) launch<__half, 64>(a, s);
+    else launch<__half, 128>(a, s);
   } else {
-    if (x->head_dim == 64) paged_append_kernel<__nv_bfloat16, 64><<<n, kThreads, 0, s>>>(a);
-    else paged_append_kernel<__nv_bfloat16, 128><<<n, kThreads, 0, s>>>(a);
+    if (x->head_dim == 64) launch<__nv_bfloat16, 64>(a, s);
+    else launch<__nv_bfloat16, 128>(a, s);
   }
   count_launch();
   return launch_status();

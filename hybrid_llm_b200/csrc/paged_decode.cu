@@ -14,7 +14,9 @@
 // the softmax and 16 x DH outputs in registers, and no barrier ties it to the
 // other warps.  A sequence-head that one worker holds whole is written at
 // once; the pieces of the others go to scratch (unnormalised sum, maximum,
-// weight sum, fp32) and a second launch joins them, in a fixed order.
+// weight sum, fp32) and a second launch joins them, in a fixed order.  Short
+// caches go without: a CTA per sequence and kv head, its four warps joined in
+// shared memory.
 #include <algorithm>
 
 #include "mma.cuh"
@@ -37,6 +39,7 @@ struct DecodeArgs {
   PagedPool pool;
   int32_t group, chunks, rows;  // heads per kv head, chunks of them, heads per chunk at most
   int32_t q_heads, window, workers;
+  int32_t whole;  // a CTA per (sequence, kv head, chunk), joined in shared memory
   float scale, softcap;
   const float* slopes;
   uint16_t* out;
@@ -138,14 +141,21 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) paged_decode_kernel(D
   const int worker = blockIdx.x * kWarps + warp;
   pdl_trigger();
   const int hcs = a.pool.kv_heads * a.chunks;
-  const int64_t tiles = total_tiles<KT>(a) * hcs;
-  const int64_t share = share_of(tiles, a.workers);
-  const int64_t t0 = worker * share, t1 = min(tiles, t0 + share);
-  if (t0 >= t1) return;
   uint8_t* ring = smem + warp * kStages * kStageBytes;
-
   Cursor ld;  // where the loads are
-  {
+  int n_load;
+  if (a.whole) {  // a quarter of one segment's tiles
+    ld.b = blockIdx.x / hcs;
+    ld.hc = blockIdx.x % hcs;
+    ld.enter<KT>(a);
+    ld.tile = warp * ld.count / kWarps;
+    n_load = (warp + 1) * ld.count / kWarps - ld.tile;
+  } else {
+    const int64_t tiles = total_tiles<KT>(a) * hcs;
+    const int64_t share = share_of(tiles, a.workers);
+    const int64_t t0 = worker * share, t1 = min(tiles, t0 + share);
+    if (t0 >= t1) return;
+    n_load = static_cast<int>(t1 - t0);
     int64_t before;
     ld.b = find_sequence<KT>(a, t0, hcs, before);
     ld.enter<KT>(a);
@@ -154,7 +164,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) paged_decode_kernel(D
     ld.tile = static_cast<int>(r % ld.count);
   }
   Cursor cu = ld;  // where the products are
-  int n_load = static_cast<int>(t1 - t0), n_left = n_load;
+  int n_left = n_load;
   int page[kPieces];  // of the next tile to load
   auto look_up = [&]() {
 #pragma unroll
@@ -231,11 +241,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) paged_decode_kernel(D
   begin();
   const float sc = a.scale * kLog2e, cap = a.softcap * kLog2e;
   const float cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
-  bool whole_start = cu.tile == 0;  // this worker holds the segment's first tile
+  bool whole_start = !a.whole && cu.tile == 0;  // this worker holds the segment's first tile
   bool first_segment = true;
   int stage = 0;
 
-  while (true) {
+  while (n_left > 0) {
     mma::cp_async_wait<kStages - 2>();
     __syncwarp();
     load(stage == 0 ? kStages - 1 : stage - 1);  // the stage read one tile ago
@@ -327,7 +337,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) paged_decode_kernel(D
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
       }
-      if (seg_end && whole_start) {
+      if (a.whole) {
+        // (joined below)
+      } else if (seg_end && whole_start) {
         const int head0 = (cu.hc / a.chunks) * a.group + (cu.hc % a.chunks) * 16;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -366,6 +378,49 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) paged_decode_kernel(D
     }
   }
   mma::cp_async_wait<0>();
+  if (!a.whole) return;
+  // the warps' pieces, through their rings
+  float* const piece = reinterpret_cast<float*>(ring);
+  float2* const piece_ml = reinterpret_cast<float2*>(ring + 16 * DH * 4);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = r0 + 8 * i;
+#pragma unroll
+    for (int n = 0; n < DH / 8; ++n)
+      *reinterpret_cast<float2*>(piece + r * DH + 8 * n + c0) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+    if ((lane & 3) == 0) piece_ml[r] = make_float2(m[i], l[i]);
+  }
+  __syncthreads();
+  const int b = blockIdx.x / hcs, hc = blockIdx.x % hcs;
+  const int head0 = (hc / a.chunks) * a.group + (hc % a.chunks) * 16;
+  for (int x = threadIdx.x; x < rows * (DH / 4); x += kWarps * 32) {
+    const int r = x / (DH / 4), c = x % (DH / 4);
+    float2 ml[kWarps];
+    float4 p[kWarps];
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const uint8_t* const from = smem + w * kStages * kStageBytes;
+      ml[w] = reinterpret_cast<const float2*>(from + 16 * DH * 4)[r];
+      p[w] = reinterpret_cast<const float4*>(from)[r * (DH / 4) + c];
+      top = fmaxf(top, ml[w].x);
+    }
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = fast_exp2(ml[w].x - base);
+      sum = fmaf(ml[w].y, f, sum);
+      y.x = fmaf(p[w].x, f, y.x), y.y = fmaf(p[w].y, f, y.y);
+      y.z = fmaf(p[w].z, f, y.z), y.w = fmaf(p[w].w, f, y.w);
+    }
+    const float inv = inv_of(sum);
+    *reinterpret_cast<uint2*>(a.out + b * a.o_tok + (head0 + r) * a.o_head + 4 * c) =
+        make_uint2(Elem<T>::pack(y.x * inv, y.y * inv), Elem<T>::pack(y.z * inv, y.w * inv));
+    if (a.lse && c == 0) a.lse[static_cast<int64_t>(b) * a.q_heads + head0 + r] = lse_of(top, sum);
+  }
 }
 
 // Joins the pieces of the sequence-heads that several workers share: one CTA
@@ -455,18 +510,32 @@ __global__ void __launch_bounds__(NT) paged_decode_join_kernel(DecodeArgs a) {
   if (a.lse && v == 0) a.lse[static_cast<int64_t>(b) * a.q_heads + head] = lse_of(m, l);
 }
 
+// One CTA per sequence and kv head instead of equal shares, by what the table
+// can hold: where that is a few tiles (the second launch costs more: 300 keys
+// of 8 heads of 64, 5.8 us against 6.3 and one launch less for the host), and
+// where there are CTAs enough to even lengths out (64 x 4 heads of 128 with
+// 1024 keys: 25.1 us against 30.8; with few CTAs uneven lengths would leave SMs idle).
+bool whole_segments(int64_t segments, int table_width, int page_size, int head_dim) {
+  const int64_t tiles = static_cast<int64_t>(table_width) * page_size / (2048 / head_dim);
+  return segments <= 0x7fffffff && (tiles <= 16 || (tiles <= 64 && segments >= 4 * num_sms()));
+}
+
 int worker_count() { return num_sms() * kCtasPerSm * kWarps; }
 
 template <typename T, int DH>
 int32_t launch(const DecodeArgs& a, cudaStream_t s) {
   int32_t st = ensure_smem(paged_decode_kernel<T, DH>, kSmem);
   if (st) return st;
-  paged_decode_kernel<T, DH><<<a.workers / kWarps, kWarps * 32, kSmem, s>>>(a);
+  const int64_t segments = static_cast<int64_t>(a.pool.batch) * a.pool.kv_heads * a.chunks;
+  paged_decode_kernel<T, DH>
+      <<<static_cast<unsigned>(a.whole ? segments : a.workers / kWarps), kWarps * 32, kSmem, s>>>(a);
   st = launch_status();
-  if (st) return st;
+  if (st || a.whole) {
+    count_launch();
+    return st;
+  }
   // Pieces per row: with few rows there are many (one sequence, 4 kv heads:
   // 296), which 128 threads would read one after another (29 us against 5).
-  const int64_t segments = static_cast<int64_t>(a.pool.batch) * a.pool.kv_heads * a.chunks;
   const dim3 grid(static_cast<unsigned>(segments * a.rows));
   const cudaError_t e =
       a.workers > 16 * segments
@@ -506,6 +575,8 @@ LLMYB_API int32_t llmyb_paged_decode(const llmyb_paged_args* x, void* stream) {
   a.chunks = (a.group + 15) / 16;
   a.rows = std::min(16, a.group);
   a.q_heads = x->q_heads, a.window = x->window, a.workers = worker_count();
+  a.whole = whole_segments(static_cast<int64_t>(x->batch) * x->kv_heads * a.chunks, x->table_width,
+                           x->page_size, x->head_dim);
   a.scale = x->scale, a.softcap = x->softcap, a.slopes = x->slopes;
   a.out = static_cast<uint16_t*>(x->out);
   a.o_tok = x->out_token_stride, a.o_head = x->out_head_stride;

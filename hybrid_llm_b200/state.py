@@ -174,3 +174,101 @@ class RecurrentState:
                 if name == "local_vo" and f"{name}.{key}" not in sd:
                     continue
                 t.copy_(sd[f"{name}.{key}"])
+
+
+class PagedKVCache:
+    """Keys and values of attention blocks that reach further than a ring of
+    ``csa_window`` rows: pages of ``page_size`` positions handed out to the rows
+    of a batch as they grow, so rows of any lengths share one memory.
+
+      * ``k[layer]`` / ``v[layer]`` [pages, kv_heads, page_size, head_dim] (bf16 or fp16)
+      * ``block_table`` [batch, max_pages] int32, the pages of every row (-1: none)
+      * ``lengths`` [batch] int32, positions of every row
+    One table serves all layers.  Pages are managed on the host (``reserve``,
+    ``extend``, ``release``); ``append`` and ``attend`` are the kernels of
+    kernels.py on one layer.  A decode step captured in a CUDA graph reserves
+    its pages before, and counts ``lengths`` up inside the graph.
+    """
+
+    def __init__(self, kv_heads: int, head_dim: int, *, batch: int, pages: int,
+                 page_size: int = 64, max_pages: int | None = None, layers: int = 1,
+                 dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda"):
+        """max_pages: pages of one row at most (default: all of them)."""
+        if page_size not in (16, 32, 64, 128, 256):
+            raise ValueError("page_size must be 16, 32, 64, 128 or 256")
+        if head_dim not in (64, 128) or dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("head dimensions 64 and 128 in bf16 or fp16 are served")
+        if kv_heads < 1 or batch < 1 or pages < 1 or layers < 1:
+            raise ValueError("kv_heads, batch, pages and layers must be positive")
+        self.batch, self.page_size = int(batch), int(page_size)
+        self.max_pages = int(pages if max_pages is None else max_pages)
+        self.device = torch.device(device)
+        shape = (int(pages), int(kv_heads), self.page_size, int(head_dim))
+        self.k = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(layers)]
+        self.v = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(layers)]
+        self.block_table = torch.full((self.batch, self.max_pages), -1, dtype=torch.int32,
+                                      device=self.device)
+        self.lengths = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
+        self._held: list[list[int]] = [[] for _ in range(self.batch)]
+        self._length = [0] * self.batch
+        self._free = list(range(int(pages) - 1, -1, -1))
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _counts(self, tokens) -> list[int]:
+        counts = [int(t) for t in tokens]
+        if len(counts) != self.batch or min(counts) < 0:
+            raise ValueError(f"one count >= 0 for each of the {self.batch} rows is needed")
+        return counts
+
+    def reserve(self, tokens) -> None:
+        """Pages for tokens[b] more positions of every row; lengths stay.  Raises
+        and changes nothing where pages run out or a row outgrows max_pages."""
+        counts = self._counts(tokens)
+        more = [max(0, -(-(n + c) // self.page_size) - len(h))
+                for n, c, h in zip(self._length, counts, self._held)]
+        if sum(more) > len(self._free):
+            raise RuntimeError(f"the cache has {len(self._free)} free pages, {sum(more)} are needed")
+        if any(len(h) + m > self.max_pages for h, m in zip(self._held, more)):
+            raise RuntimeError(f"a row has at most {self.max_pages} pages")
+        for b, m in enumerate(more):
+            if m:
+                first = len(self._held[b])
+                self._held[b] += [self._free.pop() for _ in range(m)]
+                self.block_table[b, first:first + m] = torch.tensor(
+                    self._held[b][first:], dtype=torch.int32).to(self.device)
+
+    def extend(self, tokens) -> torch.Tensor:
+        """Reserves the pages and counts the lengths up; returns cu_q [batch + 1]
+        int32, the packing of the new tokens."""
+        counts = self._counts(tokens)
+        self.reserve(counts)
+        self._length = [n + c for n, c in zip(self._length, counts)]
+        self.lengths.copy_(torch.tensor(self._length, dtype=torch.int32))
+        return torch.tensor([0, *counts], dtype=torch.int64).cumsum(0).to(torch.int32).to(self.device)
+
+    def release(self, rows) -> None:
+        """Gives the pages of the rows back; their lengths are 0."""
+        for b in {int(r) for r in rows}:
+            self._free += reversed(self._held[b])
+            self._held[b], self._length[b] = [], 0
+            self.block_table[b].fill_(-1)
+            self.lengths[b] = 0
+
+    def append(self, layer: int, q, k, v, cu_q=None, **options) -> torch.Tensor:
+        """kernels.paged_append on a layer: the new tokens' keys and values into
+        their pages, the queries back.  cu_q of extend; None: one token per row."""
+        from . import kernels
+        return kernels.paged_append(q, k, v, self.k[layer], self.v[layer], self.block_table,
+                                    self.lengths, cu_q=cu_q, **options)
+
+    def attend(self, layer: int, q, cu_q=None, **options) -> torch.Tensor:
+        """Attention of the new tokens over their rows: kernels.paged_prefill, or
+        kernels.paged_decode where cu_q is None (one token per row)."""
+        from . import kernels
+        at = (self.k[layer], self.v[layer], self.block_table, self.lengths)
+        if cu_q is None:
+            return kernels.paged_decode(q, *at, **options)
+        return kernels.paged_prefill(q, *at, cu_q, **options)

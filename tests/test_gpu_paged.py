@@ -527,3 +527,46 @@ def test_empty_calls(cuda):
     kernels.paged_prefill(row, cache.kd, cache.vd, cache.td, cache.ld, two, out=out)
     assert torch.equal(out, row)
     kernels.check_device_status()
+
+
+def test_cache_object_serves_a_batch(cuda):
+    """PagedKVCache: prompts, steps, a row that ends and another that takes its pages."""
+    from hybrid_llm_b200.state import PagedKVCache
+    hq, kv, dim = 4, 2, 64
+    c = PagedKVCache(kv, dim, batch=2, pages=12, page_size=16, layers=2)
+    g = torch.Generator().manual_seed(6)
+    rows = {0: [], 1: []}  # (key, value) of every position
+
+    def check(new, cu_q):
+        n = sum(new)
+        x = torch.randn(n, hq + 2 * kv, dim, generator=g).bfloat16().cuda()
+        for layer in range(2):
+            q = c.append(layer, x[:, :hq], x[:, hq:hq + kv], x[:, hq + kv:], cu_q)
+            out = c.attend(layer, q, cu_q)
+            if layer == 0:
+                at = 0
+                for b, t in enumerate(new):
+                    rows[b] += [(x[i, hq:hq + kv], x[i, hq + kv:]) for i in range(at, at + t)]
+                    at += t
+            at = 0
+            for b, t in enumerate(new):
+                if t == 0:
+                    continue
+                k, v = (_np(torch.stack([r[j] for r in rows[b]])) for j in (0, 1))
+                ref, mag, _ = paged.attention(
+                    _np(q[at:at + t]), k.transpose(1, 0, 2)[None], v.transpose(1, 0, 2)[None],
+                    np.zeros((1, 1), int), [len(rows[b])], [0, t], scale=dim ** -0.5)
+                _close(out[at:at + t], ref, mag, torch.bfloat16, [1], 1)
+                at += t
+
+    check([50, 20], c.extend([50, 20]))
+    for _ in range(3):
+        c.extend([1, 1])
+        check([1, 1], None)
+    check([0, 30], c.extend([0, 30]))
+    c.release([0])
+    rows[0] = []
+    check([90, 1], c.extend([90, 1]))
+    assert c.free_pages == 12 - 6 - 4
+    from hybrid_llm_b200 import kernels
+    kernels.check_device_status()

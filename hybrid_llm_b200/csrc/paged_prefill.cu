@@ -44,7 +44,7 @@ namespace {
 constexpr int kRows = 128;         // rows per tile = keys per block
 constexpr int kBox = kRows * 128;  // 128 rows x 64 elements
 constexpr int kThreads = 384;
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;  // 256 x 208 + 128 x 88 = 384 x 168
+constexpr int kSoftmaxRegs = 192, kOtherRegs = 120;  // 256 x 192 + 128 x 120 = 384 x 168
 constexpr uint32_t kTmemCols = 512;
 constexpr int kJoinThreads = 256, kJoinRows = 32;
 // What a unit costs beside its blocks (queries, first scores, the output), in blocks.
@@ -364,6 +364,19 @@ __device__ __forceinline__ void set_pair(uint32_t (&s)[128], int e, uint64_t v) 
   s[e + 1] = __float_as_uint(x.y);
 }
 
+// Elements outside [lo, hi] become `other`: a word of 32 bits per 32 elements,
+// whose bits go to predicates several at a time.
+__device__ __forceinline__ void keep(uint32_t (&s)[128], int lo, int hi, uint32_t other) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    auto ones = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
+    const uint32_t in = ones(hi + 1 - 32 * c) & ~ones(lo - 32 * c);
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if ((in & (1u << e)) == 0) s[32 * c + e] = other;
+  }
+}
+
 // largest of three, NaN if one is
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -439,13 +452,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
   const uint32_t tmem = *tmem_slot;
   int32_t* const status = a.dev_status;
   if (a.cut && threadIdx.x == 0) a.cuts[blockIdx.x] = {-1, 0, 0, 0, 0, 0};
-  // the next unit, for every role but TMA's (n: units so far)
-  auto get = [&](uint32_t n, Unit& u) -> bool {
-    if (!wait(&u_full[n & 1], (n >> 1) & 1, status, abort_flag)) return false;
-    u = ring[n & 1];
+  // the next unit, for every role but TMA's (n: units so far); it stays in the
+  // ring, out of the registers, until its role is done with it
+  auto get = [&](uint32_t n) -> bool {
+    return wait(&u_full[n & 1], (n >> 1) & 1, status, abort_flag) && ring[n & 1].blocks >= 0;
+  };
+  auto done = [&](uint32_t n) {
     __syncwarp();
     if (lane == 0) sm100::mbar_arrive(&u_empty[n & 1]);
-    return u.blocks >= 0;
   };
 
   // the register split is set inside the role branches: what follows a common
@@ -581,9 +595,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
         if (sm100::elect_one()) sm100::umma_commit(bar);
         __syncwarp();
       };
-      Unit u;
-      for (uint32_t n = 0; ok && get(n, u); ++n) {
-        const int blocks = u.blocks, tiles = u.tiles;
+      for (uint32_t n = 0; ok && get(n); ++n) {
+        const int blocks = ring[n & 1].blocks, tiles = ring[n & 1].tiles;
+        done(n);
         if (blocks == 0) continue;
         if (!(ok = wait(q_full, n_q & 1, status, abort_flag) && wait_kv(n_kv))) break;
         ++n_q;
@@ -628,10 +642,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
     const int tok = row / a.group, g = row % a.group;  // token and head within the tile
     uint32_t n_s = 0, n_o = 0;
     bool ok = true;
-    Unit u;
-    for (uint32_t n = 0; ok && get(n, u); ++n) {
-      const bool whole = u.starts && u.ends;
-      if (threadIdx.x == 0 && !whole) {
+    for (uint32_t n = 0; ok && get(n); ++n) {
+      const Unit& u = ring[n & 1];
+      if (threadIdx.x == 0 && !(u.starts && u.ends)) {
         CutUnit& cut = a.cuts[blockIdx.x];
         if (u.starts) {
           cut.slot = 1, cut.token = u.token, cut.count = u.count, cut.kvh = u.kvh;
@@ -639,7 +652,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
           cut.continues = 1, cut.ends = u.ends;
         }
       }
-      if (t >= u.tiles) continue;
+      if (t >= u.tiles) {
+        done(n);
+        continue;
+      }
+      float m = -INFINITY, l = 0.f;
+      const int blocks = u.blocks;
+      {
       const int local = t * a.tile_tokens + tok;  // within the unit
       const bool live = tok < a.tile_tokens && local < u.count;
       const int pos = u.pos + local;
@@ -653,9 +672,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
       const float slope = kBias && live ? a.slopes[u.kvh * a.group + g] * kLog2e : 0.f;
       // l: this row's weights by 2^-m; settled: every live row of the warp has
       // its first maximum
-      float m = -INFINITY, l = 0.f;
       bool settled = false;
-      const int blocks = u.blocks, kb0 = u.kb0;
+      const int kb0 = u.kb0;
+      const bool ahead = kBias && u.prefix != 0;
       for (int j = blocks - 1; j >= 0; --j) {
         if (!(ok = wait(&s_full[t], n_s & 1, status, abort_flag))) break;
         ++n_s;
@@ -673,9 +692,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
         }
         const int j0 = (kb0 + j) * kRows;
         float sc = a.scale * kLog2e;
+        const bool edge = j0 + kRows - 1 > tile_hi || j0 < tile_lo;
+        const int lo_c = lo - j0, hi_c = hi - j0;
         if constexpr (kCap) {
-          // cap tanh(s / cap): the short form while |s| < cap, which one bit of
-          // 2 s / cap tells
+          if (__builtin_expect(edge, 0)) {  // what is not visible chooses no path below
+            keep(sr, lo_c, hi_c, 0u);
+          }
+          // cap tanh(s / cap): the short form in rows with |s| < cap, which one
+          // bit of 2 s / cap tells
           const float in = 2.f * a.scale / a.softcap;
           const uint64_t in2 = make2(in, in);
           uint32_t big = 0u;
@@ -684,9 +708,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
             set_pair(sr, e, mul2(pair(sr, e), in2));
             big |= sr[e] | sr[e + 1];
           }
-          if (__builtin_expect(__any_sync(0xffffffffu, big & 0x40000000u), 0)) {
+          const bool wide = live && (big & 0x40000000u);
+          if (__builtin_expect(__any_sync(0xffffffffu, wide), 0)) {
 #pragma unroll
-            for (int e = 0; e < 128; e += 2) set_pair(sr, e, tanh_half2(pair(sr, e)));
+            for (int e = 0; e < 128; e += 2) {
+              const uint64_t y = pair(sr, e);
+              set_pair(sr, e, wide ? tanh_half2(y) : tanh_half_poly2(y));
+            }
           } else {
 #pragma unroll
             for (int e = 0; e < 128; e += 2) set_pair(sr, e, tanh_half_poly2(pair(sr, e)));
@@ -695,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
         }
         if constexpr (kBias) {
           const float d0 = static_cast<float>(pos - j0);
-          if (u.prefix == 0 || j0 + kRows - 1 <= first_pos) {  // no visible key is ahead
+          if (!ahead || j0 + kRows - 1 <= first_pos) {  // no visible key is ahead
             const uint64_t step = make2(slope, slope), sc2 = make2(sc, sc);
             const uint64_t b0 = make2(-slope * d0, -slope * d0);
 #pragma unroll
@@ -710,13 +738,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
           }
           sc = 1.f;
         }
-        if (__builtin_expect(j0 + kRows - 1 > tile_hi || j0 < tile_lo, 0)) {
-          const int lo_c = lo - j0, hi_c = hi - j0;
-#pragma unroll
-          for (int e = 0; e < 128; ++e)
-            if (e < lo_c || e > hi_c) sr[e] = __float_as_uint(-INFINITY);
-        }
-        auto raise = [&]() {  // m to the block's maximum, l and O rescaled
+        if (__builtin_expect(edge, 0)) keep(sr, lo_c, hi_c, 0xff800000u);  // -inf
+        // m of the rows that ask for it (and of no other: a row's result does not
+        // depend on its neighbours) to the block's maximum, l and O rescaled
+        auto raise = [&](bool ask) {
           float mx[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sr[e]);
@@ -729,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
           mx[1] = max3(mx[1], __uint_as_float(sr[126]), __uint_as_float(sr[127]));
           const float bm = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * sc;
           float alpha = 1.f;
-          if (bm > m) {
+          if (ask && bm > m) {
             alpha = fast_exp2(m - bm);
             m = bm;
             l *= alpha;
@@ -774,12 +799,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
         // formed (459 us against 502 with it).  Else, a NaN among them
         // included, and at a row's first keys it is.
         if (!settled) {
-          if (__any_sync(0xffffffffu, live && m == -INFINITY && hi >= j0)) raise();
+          const bool fresh = live && m == -INFINITY && hi >= j0;
+          if (__any_sync(0xffffffffu, fresh)) raise(fresh);
           settled = __all_sync(0xffffffffu, !live || m != -INFINITY);
         }
         float sum = weights();
-        if (__builtin_expect(__any_sync(0xffffffffu, !(sum <= 16384.f)), 0)) {
-          raise();
+        const bool far = live && !(sum <= 16384.f);
+        if (__builtin_expect(__any_sync(0xffffffffu, far), 0)) {
+          raise(far);
           sum = weights();
         }
         l += sum;
@@ -788,6 +815,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(&p_full[t]);
       }
+      }
       if (!ok) break;
       // ---------------------------------------------------- epilogue
       if (blocks > 0) {
@@ -795,7 +823,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
         ++n_o;
         sm100::tc_fence_after();
       }
+      const int local = t * a.tile_tokens + tok;
+      const bool live = tok < a.tile_tokens && local < u.count;
       const float inv = inv_of(l);
+      const bool whole = u.starts && u.ends;
       const int head = u.kvh * a.group + g;
       // This row's place in the output; the rows go there by way of shared
       // memory, 64 columns at a time, so that a store instruction writes whole
@@ -805,42 +836,46 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
       float4* const part = reinterpret_cast<float4*>(a.part_o) +
                            (2ll * blockIdx.x + (u.starts ? 1 : 0)) * (256 * D / 4) + t * kRows + row;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        if (blocks > 0) {
-          sm100::tmem_ld_32x32b_x32(t_o + 32 * c, o);
-          sm100::tmem_ld_wait();
-          sm100::tmem_regs_ready(o);
-        } else {
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t o[2][32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        for (int h = 0; h < 2; ++h) sm100::tmem_ld_32x32b_x32(t_o + 64 * c + 32 * h, o[h]);
+        sm100::tmem_ld_wait();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) sm100::tmem_regs_ready(o[h]);
+        if (blocks == 0) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) o[e / 32][e % 32] = 0u;
         }
         if (!whole) {  // column quads by row: the lanes' 16 bytes are neighbours
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            part[(8 * c + e) * 256] =
-                make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
-                            __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+          for (int e = 0; e < 16; ++e)
+            part[(16 * c + e) * 256] = make_float4(
+                __uint_as_float(o[e / 8][4 * (e % 8)]), __uint_as_float(o[e / 8][4 * (e % 8) + 1]),
+                __uint_as_float(o[e / 8][4 * (e % 8) + 2]), __uint_as_float(o[e / 8][4 * (e % 8) + 3]));
           continue;
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 8; ++e) {
           uint32_t w[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            w[k] = Elem<T>::pack(__uint_as_float(o[8 * e + 2 * k]) * inv,
-                                 __uint_as_float(o[8 * e + 2 * k + 1]) * inv);
-          *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c & 1) * 4 + e) ^ (lane & 7)) << 4)) =
+            w[k] = Elem<T>::pack(__uint_as_float(o[e / 4][8 * (e % 4) + 2 * k]) * inv,
+                                 __uint_as_float(o[e / 4][8 * (e % 4) + 2 * k + 1]) * inv);
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) =
               make_uint4(w[0], w[1], w[2], w[3]);
         }
-        if ((c & 1) == 0) continue;
         __syncwarp();
+        uint4 v[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int r = 4 * k + (lane >> 3);
-          const int64_t at = __shfl_sync(0xffffffffu, dst, r);
-          const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-          if (at >= 0) *reinterpret_cast<uint4*>(a.out + at + 32 * (c - 1) + 8 * (lane & 7)) = v;
+          v[k] = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int64_t at = __shfl_sync(0xffffffffu, dst, 4 * k + (lane >> 3));
+          if (at >= 0) *reinterpret_cast<uint4*>(a.out + at + 64 * c + 8 * (lane & 7)) = v[k];
         }
         __syncwarp();
       }
@@ -851,6 +886,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
           a.lse[static_cast<int64_t>(u.token + local) * a.q_heads + head] = lse_of(m, l);
       }
       sm100::tc_fence_before();  // O is read before the next unit's first product
+      done(n);
     }
   }
   sm100::tc_fence_before();
@@ -897,17 +933,26 @@ __global__ void __launch_bounds__(kJoinThreads) paged_prefill_join_kernel(Prefil
       l = fmaf(ml.y, fast_exp2(ml.x - base), l);
     }
     const float inv = inv_of(l);
-    for (int v = warp; v < D / 4; v += kWarps) {
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int c = blockIdx.x; c < end; ++c) {
-        const float f = fast_exp2(a.part_ml[slot(c) * 256 + r].x - base);
-        const float4 x = reinterpret_cast<const float4*>(a.part_o)[(slot(c) * (D / 4) + v) * 256 + r];
-        o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y);
-        o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
+    constexpr int kQuads = D / 4 / kWarps;  // column quads of this thread
+    float4 o[kQuads];
+#pragma unroll
+    for (int k = 0; k < kQuads; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+    for (int c = blockIdx.x; c < end; ++c) {
+      const float f = fast_exp2(a.part_ml[slot(c) * 256 + r].x - base);
+      const float4* const from =
+          reinterpret_cast<const float4*>(a.part_o) + (slot(c) * (D / 4) + warp) * 256 + r;
+#pragma unroll
+      for (int k = 0; k < kQuads; ++k) {
+        const float4 x = from[k * kWarps * 256];
+        o[k].x = fmaf(x.x, f, o[k].x), o[k].y = fmaf(x.y, f, o[k].y);
+        o[k].z = fmaf(x.z, f, o[k].z), o[k].w = fmaf(x.w, f, o[k].w);
       }
-      s_out[lane][v] = make_uint2(Elem<T>::pack(o.x * inv, o.y * inv), Elem<T>::pack(o.z * inv, o.w * inv));
     }
+#pragma unroll
+    for (int k = 0; k < kQuads; ++k)
+      s_out[lane][warp + k * kWarps] = make_uint2(Elem<T>::pack(o[k].x * inv, o[k].y * inv),
+                                                  Elem<T>::pack(o[k].z * inv, o[k].w * inv));
     if (warp == 0 && a.lse)
       a.lse[static_cast<int64_t>(u.token + tok) * a.q_heads + u.kvh * a.group + r % kRows % a.group] =
           lse_of(m, l);

@@ -570,3 +570,104 @@ def test_cache_object_serves_a_batch(cuda):
     assert c.free_pages == 12 - 6 - 4
     from hybrid_llm_b200 import kernels
     kernels.check_device_status()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,page", [(128, 64), (64, 16)])
+def test_decode_one_cta_per_head(cuda, dtype, dim, page):
+    """Enough rows that every sequence and kv head has a CTA of its own."""
+    from hybrid_llm_b200 import kernels
+    rng = np.random.default_rng(dim)
+    lengths = [0, 1, 800] + [int(x) for x in rng.integers(0, 700, 160)]
+    cache = Cache(lengths, 4, dim, page, DT[dtype], seed=60, pad=0)
+    q = torch.randn(len(lengths), 12, dim, device="cuda").to(DT[dtype])
+    lse = torch.empty(len(lengths), 12, device="cuda")
+    out = kernels.paged_decode(q, cache.kd, cache.vd, cache.td, cache.ld, lse=lse, window=300)
+    kernels.check_device_status()
+    _check(out, lse, cache, q, np.arange(len(lengths) + 1), DT[dtype], window=300)
+
+
+def test_tables_with_a_row_stride(cuda):
+    """block_table a slice of a wider table, through all three calls."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([70, 9], 2, 64, 16, torch.bfloat16, seed=61, pad=0)
+    wide = torch.full((2, cache.table.shape[1] + 5), -9, dtype=torch.int32, device="cuda")
+    table = wide[:, 3:3 + cache.table.shape[1]]
+    table.copy_(cache.td)
+    x = torch.randn(2, 8, 64, device="cuda").bfloat16()
+    q = kernels.paged_append(x[:, :4], x[:, 4:6], x[:, 6:], cache.kd, cache.vd, table, cache.ld)
+    for b, n in enumerate((70, 9)):
+        p, r = cache.table[b, (n - 1) // 16], (n - 1) % 16
+        cache.k_ref[p, :, r], cache.v_ref[p, :, r] = _np(x[b, 4:6]), _np(x[b, 6:])
+    cu = torch.arange(3, dtype=torch.int32, device="cuda")
+    for out in (kernels.paged_decode(q, cache.kd, cache.vd, table, cache.ld),
+                kernels.paged_prefill(q, cache.kd, cache.vd, table, cache.ld, cu)):
+        _check(out, None, cache, q, np.arange(3), torch.bfloat16)
+    kernels.check_device_status()
+
+
+@pytest.mark.parametrize("width", [2, 40])
+def test_prefill_of_very_many_sequences(cuda, width):
+    """20,000 sequences of one token (several chunk sums share one): as decode."""
+    from hybrid_llm_b200 import kernels
+    g = torch.Generator(device="cuda").manual_seed(7)
+    b, pages = 20000, 64
+    kp, vp = (torch.randn(pages, 1, 16, 64, generator=g, device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn(b, 1, 64, generator=g, device="cuda").bfloat16()
+    table = torch.randint(0, pages, (b, width), generator=g, device="cuda", dtype=torch.int32)
+    lengths = torch.randint(0, 33, (b,), generator=g, device="cuda", dtype=torch.int32)
+    cu = torch.arange(b + 1, dtype=torch.int32, device="cuda")
+    a = kernels.paged_prefill(q, kp, vp, table, lengths, cu)
+    d = kernels.paged_decode(q, kp, vp, table, lengths)
+    kernels.check_device_status()
+    # both round their weights and outputs: twice 2^-8 of each, values up to 6
+    assert (a.float() - d.float()).abs().max() <= 4 * 2.0 ** -8 * 6
+    # the mean over 1.2 million values is unbiased, so a lost sequence shows
+    assert (a.float() - d.float()).abs().mean() < 2.0 ** -8
+    assert (a[lengths == 0] == 0).all()
+
+
+def test_prefill_many_groups_of_sequences(cuda):
+    """75 sequences in three groups, pieces in several chunks, some empty."""
+    from hybrid_llm_b200 import kernels
+    rng = np.random.default_rng(8)
+    new = [int(x) for x in rng.integers(0, 60, 75)]
+    new[3], new[40], new[74] = 700, 0, 333
+    context = [int(x) for x in rng.integers(0, 900, 75)]
+    lengths = [a + c for a, c in zip(new, context)]
+    cache = Cache(lengths, 2, 64, 32, torch.bfloat16, seed=62)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    q = torch.randn(cu[-1], 14, 64, device="cuda").bfloat16()
+    lse = torch.empty(cu[-1], 14, device="cuda")
+    out = kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld,
+                                torch.from_numpy(cu.astype(np.int32)).cuda(), lse=lse, softcap=8.0)
+    kernels.check_device_status()
+    _check(out, lse, cache, q, cu, torch.bfloat16, softcap=8.0)
+
+
+def test_non_finite_values_reach_only_their_readers(cuda):
+    """A NaN or an infinity in a query or a key spoils that row (or the rows that
+    see the key), in decode and prefill; nothing else."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([200, 300], 1, 64, 16, torch.bfloat16, seed=63)
+    new = [40, 300]
+    cu = np.concatenate([[0], np.cumsum(new)])
+    cud = torch.from_numpy(cu.astype(np.int32)).cuda()
+    q = torch.randn(cu[-1], 2, 64, device="cuda").bfloat16()
+    clean = kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld, cud)
+    bad = q.clone()
+    bad[17, 1, 5] = float("nan")
+    out = kernels.paged_prefill(bad, cache.kd, cache.vd, cache.td, cache.ld, cud)
+    assert out[17, 1].isnan().all()
+    keep = torch.ones(cu[-1], 2, dtype=torch.bool, device="cuda")
+    keep[17, 1] = False
+    assert torch.equal(out[keep], clean[keep])
+    kd = cache.kd.clone()
+    kd[cache.table[1, 250 // 16], 0, 250 % 16, 3] = float("nan")
+    for softcap in (0.0, 20.0):
+        clean = kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld, cud, softcap=softcap)
+        out = kernels.paged_prefill(q, kd, cache.vd, cache.td, cache.ld, cud, softcap=softcap)
+        assert torch.equal(out[:40 + 250], clean[:40 + 250]) and out[40 + 250:].isnan().all()
+        one = kernels.paged_decode(q[:2], kd, cache.vd, cache.td, cache.ld, softcap=softcap)
+        assert not one[0].isnan().any() and one[1].isnan().all()
+    kernels.check_device_status()

@@ -49,11 +49,11 @@ template <typename T, int DH, int kRounds>
 __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(AppendArgs a, Parts parts) {
   constexpr int kLanes = DH / 8, kHeads = 32 / kLanes;
   const int lane = threadIdx.x & 31, l = lane % kLanes;
-  const int64_t w = blockIdx.x * static_cast<int64_t>(kThreads / 32) + (threadIdx.x >> 5);
-  const int per = parts.q + 2 * parts.kv;
-  const int tok = static_cast<int>(w / per);
+  // eight tokens' part of one kind per CTA; the parts of a token are neighbours
+  const unsigned per = parts.q + 2 * parts.kv;
+  const int tok = static_cast<int>(blockIdx.x / per) * (kThreads / 32) + (threadIdx.x >> 5);
   if (tok >= a.n_tokens) return;
-  int part = static_cast<int>(w % per);
+  int part = static_cast<int>(blockIdx.x % per);
   const int kind = part < parts.q ? 0 : part < parts.q + parts.kv ? 1 : 2;
   part -= kind == 0 ? 0 : kind == 1 ? parts.q : parts.q + parts.kv;
   const int heads = kind == 0 ? a.q_heads : a.pool.kv_heads;
@@ -207,16 +207,15 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(AppendArgs a,
 
 // Rounds per warp: one where that many warps do not fill the GPU's 64 per SM
 // (a token's latency counts), else eight, so that a token's lookups and angles
-// serve several heads: 14117 tokens of 16 + 2 x 16 heads, 347 MB, take 77 us
-// (0.69 of the copy rate) with eight, 85 us with four; one CTA per token with
-// the angles in shared memory took 129 us.
+// serve several heads: 14117 tokens of 16 + 2 x 16 heads, 347 MB, take 70 us
+// (0.76 of the copy rate).  Four rounds took 85 us where eight took 77; a CTA
+// per token with the angles in shared memory, 129 us.
 template <typename T, int DH, int kRounds>
 void launch(const AppendArgs& a, cudaStream_t s) {
   constexpr int kHeads = kRounds * (256 / DH);
   const Parts p = {(a.q_heads + kHeads - 1) / kHeads, (a.pool.kv_heads + kHeads - 1) / kHeads};
-  const int64_t warps = static_cast<int64_t>(a.n_tokens) * (p.q + 2 * p.kv);
-  paged_append_kernel<T, DH, kRounds>
-      <<<static_cast<unsigned>(ceil_div(warps, kThreads / 32)), kThreads, 0, s>>>(a, p);
+  const int64_t ctas = ceil_div(a.n_tokens, kThreads / 32) * (p.q + 2 * p.kv);
+  paged_append_kernel<T, DH, kRounds><<<static_cast<unsigned>(ctas), kThreads, 0, s>>>(a, p);
 }
 template <typename T, int DH>
 void launch(const AppendArgs& a, cudaStream_t s) {

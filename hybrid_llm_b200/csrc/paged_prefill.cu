@@ -1059,6 +1059,9 @@ LLMYB_API int32_t llmyb_paged_prefill(const llmyb_paged_args* x, void* stream) {
   if (!x->cu_q) return LLMYB_EINVAL;
   const int group = x->q_heads / x->kv_heads;
   if (group > kRows || !paged_aligned(x->scratch)) return LLMYB_EUNSUPPORTED;
+  // the weights of 32 pieces are added in 32 bits
+  const int64_t blocks = ceil_div(static_cast<int64_t>(x->table_width) * x->page_size, kRows);
+  if ((blocks + kUnitCost) * x->kv_heads >= 1ll << 26) return LLMYB_EUNSUPPORTED;
   PrefillArgs a;
   a.pool = paged_pool(x);
   a.cu_q = x->cu_q, a.prefix = x->prefix, a.n_tokens = x->n_tokens, a.q_heads = x->q_heads;

@@ -852,7 +852,9 @@ int32_t llmyb_paged_decode(const llmyb_paged_args* args, void* stream);
  * (window > 0) i - j < window, or (prefix, not together with a window)
  * j < prefix[b].  Rows that see no key give zeros.  Values of visible 128-key
  * blocks must be finite (rows outside the sequence may hold anything).
- * q_heads / kv_heads <= 128; scratch may be null where scratch_bytes is 0. */
+ * q_heads / kv_heads <= 128; kv_heads times the 128-key blocks that the table
+ * can hold at most 2^26 (LLMYB_EUNSUPPORTED); scratch may be null where
+ * scratch_bytes is 0. */
 int64_t llmyb_paged_prefill_scratch_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                                           int32_t table_width, int32_t page_size);
 int32_t llmyb_paged_prefill(const llmyb_paged_args* args, void* stream);

@@ -347,11 +347,15 @@ struct Units {
 // A wait that polls: the suspending wait of sm100.cuh wakes up to a
 // microsecond late, which the chain S -> P -> O pays twice per block
 // (prefill of 8192 tokens: 769 us with it, 614 us polling).  Bounded like it.
+// Every lane waits for itself: a phase that one lane has seen complete stays so
+// until its warp goes on, so the lanes agree without a vote (which cost 4 %);
+// after another role's timeout a late completion counts as none.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int32_t* status,
                                      volatile int* abort_flag) {
   for (int i = 0; i < 4096; ++i)
     if (sm100::mbar_try_wait(bar, parity)) return true;
-  return sm100::mbar_wait_warp(bar, parity, status, abort_flag);
+  return sm100::mbar_wait(bar, parity, status, abort_flag) &&
+         (abort_flag == nullptr || !*abort_flag);
 }
 
 // elements e and e + 1 of a row of scores
@@ -656,9 +660,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
         done(n);
         continue;
       }
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f;  // l: this row's weights by 2^-m
       const int blocks = u.blocks;
-      {
       const int local = t * a.tile_tokens + tok;  // within the unit
       const bool live = tok < a.tile_tokens && local < u.count;
       const int pos = u.pos + local;
@@ -670,9 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
       const int tile_hi = first_pos < 0 ? -1 : max(first_pos, u.prefix - 1);
       const int tile_lo = a.window > 0 ? first_pos + a.tile_tokens - a.window : 0;
       const float slope = kBias && live ? a.slopes[u.kvh * a.group + g] * kLog2e : 0.f;
-      // l: this row's weights by 2^-m; settled: every live row of the warp has
-      // its first maximum
-      bool settled = false;
+      bool settled = false;  // every live row of the warp has its first maximum
       const int kb0 = u.kb0;
       const bool ahead = kBias && u.prefix != 0;
       for (int j = blocks - 1; j >= 0; --j) {
@@ -815,7 +816,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(&p_full[t]);
       }
-      }
       if (!ok) break;
       // ---------------------------------------------------- epilogue
       if (blocks > 0) {
@@ -823,8 +823,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
         ++n_o;
         sm100::tc_fence_after();
       }
-      const int local = t * a.tile_tokens + tok;
-      const bool live = tok < a.tile_tokens && local < u.count;
       const float inv = inv_of(l);
       const bool whole = u.starts && u.ends;
       const int head = u.kvh * a.group + g;

@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
       const bool live = tok < a.tile_tokens && local < u.count;
       const int pos = u.pos + local;
       // visible keys of this row: lo <= j <= hi
-      const int lo = a.window > 0 ? pos - a.window + 1 : 0;
+      const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
       const int hi = pos < 0 ? -1 : max(pos, u.prefix - 1);
       // of every row of the tile: max lo, min hi
       const int first_pos = u.pos + t * a.tile_tokens;

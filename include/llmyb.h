@@ -789,7 +789,8 @@ int32_t llmyb_decode_persistent(const llmyb_pdecode* p, void* stream);
  * elements (any order, the head dimension contiguous; both pools alike).
  * table[b * table_stride + i] (i < table_width) is the page of positions
  * [i * page_size, (i + 1) * page_size) of sequence b; lengths[b] counts its
- * positions, the new ones included.  page_size 16, 32, 64, 128 or 256;
+ * positions, the new ones included (beyond table_width * page_size, attention
+ * counts that many; append reports the token).  page_size 16, 32, 64, 128 or 256;
  * head_dim 64 or 128; q_heads a multiple of kv_heads (query head h reads kv
  * head h / (q_heads / kv_heads)).  Row tensors are [token][head][head_dim]
  * with token and head strides; pointers 16-byte aligned, strides multiples of

@@ -671,3 +671,35 @@ def test_non_finite_values_reach_only_their_readers(cuda):
         one = kernels.paged_decode(q[:2], kd, cache.vd, cache.td, cache.ld, softcap=softcap)
         assert not one[0].isnan().any() and one[1].isnan().all()
     kernels.check_device_status()
+
+
+def test_largest_window_and_lengths_beyond_the_table(cuda):
+    """A window of 2^31 - 1 is none; attention counts what the table holds, append
+    reports a token that has no page."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([64, 700], 2, 128, 16, torch.bfloat16, seed=64, pad=0)
+    # the shorter row's table is filled up so that every position has a page
+    cache.table[0] = np.where(cache.table[0] < 0, cache.table[1], cache.table[0])
+    td = torch.from_numpy(cache.table).cuda()
+    held = cache.table.shape[1] * 16
+    cu = torch.tensor([0, 3, 40], dtype=torch.int32, device="cuda")
+    q = torch.randn(40, 4, 128, device="cuda").bfloat16()
+    w = 2 ** 31 - 1
+    assert torch.equal(kernels.paged_prefill(q, cache.kd, cache.vd, td, cache.ld, cu, window=w),
+                       kernels.paged_prefill(q, cache.kd, cache.vd, td, cache.ld, cu))
+    assert torch.equal(kernels.paged_decode(q[:2], cache.kd, cache.vd, td, cache.ld, window=w),
+                       kernels.paged_decode(q[:2], cache.kd, cache.vd, td, cache.ld))
+    kernels.check_device_status()
+    kd, vd = cache.kd.nan_to_num(0, 0, 0), cache.vd.nan_to_num(0, 0, 0)
+    full = torch.tensor([held, held], dtype=torch.int32, device="cuda")
+    beyond = torch.tensor([held + 1, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    assert torch.equal(kernels.paged_decode(q[:2], kd, vd, td, beyond),
+                       kernels.paged_decode(q[:2], kd, vd, td, full))
+    assert torch.equal(kernels.paged_prefill(q, kd, vd, td, beyond, cu),
+                       kernels.paged_prefill(q, kd, vd, td, full, cu))
+    kernels.check_device_status()
+    before = kd.clone()
+    kernels.paged_append(q[:2], q[:2, :2], q[:2, :2], kd, vd, td, beyond)
+    with pytest.raises(RuntimeError, match="invalid argument"):
+        kernels.check_device_status()
+    assert torch.equal(kd, before)

@@ -186,8 +186,13 @@ class PagedKVCache:
       * ``lengths`` [batch] int32, positions of every row
     One table serves all layers.  Pages are managed on the host (``reserve``,
     ``extend``, ``release``); ``append`` and ``attend`` are the kernels of
-    kernels.py on one layer.  A decode step captured in a CUDA graph reserves
-    its pages before, and counts ``lengths`` up inside the graph.
+    kernels.py on one layer.
+
+    A decode step captured in a CUDA graph counts ``lengths`` up inside the graph
+    (``lengths.add_(live)``, live [batch] int32: 1 for the rows that go on, 0 for
+    released ones).  Its pages are reserved before the replays, and ``advance``
+    tells the host afterwards how many tokens they added: the device's lengths
+    are never overwritten by the host's, and pages are handed out by the host's.
     """
 
     def __init__(self, kv_heads: int, head_dim: int, *, batch: int, pages: int,
@@ -241,13 +246,25 @@ class PagedKVCache:
                     self._held[b][first:], dtype=torch.int32).to(self.device)
 
     def extend(self, tokens) -> torch.Tensor:
-        """Reserves the pages and counts the lengths up; returns cu_q [batch + 1]
-        int32, the packing of the new tokens."""
+        """Reserves the pages and counts the lengths up, the host's and the
+        device's; returns cu_q [batch + 1] int32, the packing of the new tokens."""
         counts = self._counts(tokens)
         self.reserve(counts)
         self._length = [n + c for n, c in zip(self._length, counts)]
-        self.lengths.copy_(torch.tensor(self._length, dtype=torch.int32))
-        return torch.tensor([0, *counts], dtype=torch.int64).cumsum(0).to(torch.int32).to(self.device)
+        cu_q = torch.tensor([0, *counts], dtype=torch.int64).cumsum(0).to(torch.int32).to(self.device)
+        self.lengths.add_(cu_q[1:] - cu_q[:-1])
+        return cu_q
+
+    def advance(self, tokens) -> None:
+        """Counts the host's lengths up by tokens that captured steps have already
+        counted on the device.  Raises and changes nothing where a row would
+        outgrow its reserved pages (its last tokens were not stored)."""
+        counts = self._counts(tokens)
+        length = [n + c for n, c in zip(self._length, counts)]
+        for b, (n, held) in enumerate(zip(length, self._held)):
+            if n > len(held) * self.page_size:
+                raise RuntimeError(f"row {b} has {len(held)} pages reserved, {n} positions need more")
+        self._length = length
 
     def release(self, rows) -> None:
         """Gives the pages of the rows back; their lengths are 0."""

@@ -703,3 +703,79 @@ def test_largest_window_and_lengths_beyond_the_table(cuda):
     with pytest.raises(RuntimeError, match="invalid argument"):
         kernels.check_device_status()
     assert torch.equal(kd, before)
+
+
+def test_captured_step_of_the_cache_object(cuda):
+    """Prompts, a captured append + attend that counts the lengths up, advance, a
+    row released, another one extended, and the same graph again."""
+    from hybrid_llm_b200 import kernels
+    from hybrid_llm_b200.state import PagedKVCache
+    hq, kv, dim, b = 4, 2, 64, 3
+    c = PagedKVCache(kv, dim, batch=b, pages=24, page_size=16)
+    kernels.device_status(c.device)
+    g = torch.Generator().manual_seed(9)
+    rows = [[] for _ in range(b)]  # (key, value) of every position
+
+    def tokens(n):
+        return torch.randn(n, hq + 2 * kv, dim, generator=g).bfloat16().cuda()
+
+    def split(x):
+        return x[:, :hq], x[:, hq:hq + kv], x[:, hq + kv:]
+
+    def check(out, x, new):
+        at = 0
+        for r, t in enumerate(new):
+            rows[r] += [(x[i, hq:hq + kv], x[i, hq + kv:]) for i in range(at, at + t)]
+            if t:
+                k, v = (_np(torch.stack([p[j] for p in rows[r]])) for j in (0, 1))
+                ref, mag, _ = paged.attention(
+                    _np(x[at:at + t, :hq]), k.transpose(1, 0, 2)[None], v.transpose(1, 0, 2)[None],
+                    np.zeros((1, 1), int), [len(rows[r])], [0, t], scale=dim ** -0.5)
+                _close(out[at:at + t], ref, mag, torch.bfloat16, [1], 1)
+            at += t
+
+    def prompt(new):
+        cu, x = c.extend(new), tokens(sum(new))
+        q, k, v = split(x)
+        check(c.attend(0, c.append(0, q, k, v, cu), cu), x, new)
+
+    prompt([20, 5, 40])
+    x = tokens(b)
+    live = torch.zeros(b, dtype=torch.int32, device="cuda")
+    c.extend([1, 1, 1])
+    q, k, v = split(x)
+    check(c.attend(0, c.append(0, q, k, v)), x.clone(), [1, 1, 1])
+
+    def step():
+        c.lengths.add_(live)
+        q, k, v = split(x)
+        return c.attend(0, c.append(0, q, k, v))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = step()
+
+    def replay(times, new):
+        c.reserve([times * n for n in new])
+        live.copy_(torch.tensor(new, dtype=torch.int32))
+        for _ in range(times):
+            x.copy_(tokens(b))
+            graph.replay()
+            for r, n in enumerate(new):
+                if n == 0:
+                    assert (out[r] == 0).all()
+            keep = [r for r in range(b) if new[r]]
+            check(out[keep], x[keep], new)
+        c.advance([times * n for n in new])
+
+    replay(12, [1, 1, 1])
+    assert c.lengths.tolist() == [33, 18, 53]
+    prompt([0, 7, 0])
+    c.release([0])
+    rows[0] = []
+    replay(20, [0, 1, 1])
+    prompt([33, 1, 2])
+    replay(3, [1, 1, 1])
+    assert c.lengths.tolist() == [36, 49, 78]
+    kernels.check_device_status()

@@ -189,3 +189,49 @@ def test_released_pages_come_back():
 def test_cache_refusals(over):
     with pytest.raises(ValueError):
         _cache(**over)
+
+
+def test_lengths_counted_on_the_device_are_kept():
+    """Steps that count the device's lengths up (a captured graph), told to the host
+    by advance: extend goes on from them and reserve counts pages from them."""
+    c = _cache(pages=16)
+    c.extend([20, 5, 0])
+    c.reserve([10, 10, 0])
+    live = torch.tensor([1, 1, 0], dtype=torch.int32)
+    for _ in range(10):
+        c.lengths.add_(live)
+    c.advance([10, 10, 0])
+    assert c.lengths.tolist() == [30, 15, 0]
+    assert c.extend([0, 7, 0]).tolist() == [0, 0, 7, 7]
+    assert c.lengths.tolist() == [30, 22, 0] and [len(r) for r in _rows(c)] == [2, 2, 0]
+    c.reserve([20, 0, 0])                            # positions 30 .. 49: two more pages
+    assert [len(r) for r in _rows(c)] == [4, 2, 0]
+    c.release([0])
+    assert c.extend([3, 1, 0]).tolist() == [0, 3, 4, 4] and c.lengths.tolist() == [3, 23, 0]
+
+
+def test_device_lengths_are_not_rewound():
+    """Before advance is called, extend keeps what the device has counted."""
+    c = _cache()
+    c.extend([10, 0, 0])
+    c.reserve([20, 0, 0])
+    c.lengths[0] += 20
+    c.extend([1, 0, 0])
+    assert c.lengths.tolist() == [31, 0, 0]
+
+
+def test_advance_refuses_what_has_no_page():
+    c = _cache()
+    c.extend([10, 3, 0])
+    c.reserve([7, 0, 0])
+    state = _rows(c), c.lengths.tolist(), c.free_pages
+    for tokens in ([23, 0, 0], [0, 14, 0], [0, 0, 1]):
+        with pytest.raises(RuntimeError, match="reserved"):
+            c.advance(tokens)
+    for tokens in ([1, 1], [1, -1, 0]):
+        with pytest.raises(ValueError):
+            c.advance(tokens)
+    assert (_rows(c), c.lengths.tolist(), c.free_pages) == state
+    c.advance([22, 13, 0])
+    c.reserve([1, 1, 0])
+    assert [len(r) for r in _rows(c)] == [3, 2, 0]

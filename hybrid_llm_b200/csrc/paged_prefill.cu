@@ -107,6 +107,13 @@ struct Seq {
   }
 };
 
+// First key that the window leaves to a token at `pos`.  Positions go down to
+// minus the token count (a length shorter than its tokens) and the window up to
+// 2^31 - 1, so their difference is formed from position 0 on.
+__device__ __forceinline__ int first_key(const PrefillArgs& a, int pos) {
+  return a.window > 0 ? max(0, max(pos, 0) - a.window + 1) : 0;
+}
+
 // Key blocks [kb0, kb0 + count) that the tokens of one piece see.
 __device__ __forceinline__ int piece_blocks(const PrefillArgs& a, const Seq& s, int piece, int& kb0,
                                             int& lo) {
@@ -114,7 +121,7 @@ __device__ __forceinline__ int piece_blocks(const PrefillArgs& a, const Seq& s, 
   const int last = pos + min(2 * a.tile_tokens, s.n - t0) - 1;
   int hi = last + 1;
   if (last >= 0) hi = max(hi, s.prefix);
-  lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+  lo = first_key(a, pos);
   kb0 = lo / kRows;
   return max(0, (hi + kRows - 1) / kRows - kb0);
 }
@@ -666,12 +673,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
       const bool live = tok < a.tile_tokens && local < u.count;
       const int pos = u.pos + local;
       // visible keys of this row: lo <= j <= hi
-      const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+      const int lo = first_key(a, pos);
       const int hi = pos < 0 ? -1 : max(pos, u.prefix - 1);
       // of every row of the tile: max lo, min hi
       const int first_pos = u.pos + t * a.tile_tokens;
       const int tile_hi = first_pos < 0 ? -1 : max(first_pos, u.prefix - 1);
-      const int tile_lo = a.window > 0 ? first_pos + a.tile_tokens - a.window : 0;
+      const int tile_lo = first_key(a, first_pos + a.tile_tokens - 1);
       const float slope = kBias && live ? a.slopes[u.kvh * a.group + g] * kLog2e : 0.f;
       bool settled = false;  // every live row of the warp has its first maximum
       const int kb0 = u.kb0;

@@ -779,3 +779,20 @@ def test_captured_step_of_the_cache_object(cuda):
     replay(3, [1, 1, 1])
     assert c.lengths.tolist() == [36, 49, 78]
     kernels.check_device_status()
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 70, 100])
+def test_prefill_window_where_tokens_have_no_position(cuda, window):
+    """A piece that begins before position 0, under the largest windows: its later
+    tokens see their keys."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([4, 0, 130], 1, 64, 16, torch.bfloat16, seed=65)
+    new = [10, 5, 140]
+    cu = np.concatenate([[0], np.cumsum(new)])
+    q = torch.randn(cu[-1], 2, 64, device="cuda").bfloat16()
+    lse = torch.empty(cu[-1], 2, device="cuda")
+    out = kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld,
+                                torch.from_numpy(cu.astype(np.int32)).cuda(), window=window, lse=lse)
+    kernels.check_device_status()
+    _check(out, lse, cache, q, cu, torch.bfloat16, window=window)
+    assert (out[:6] == 0).all() and (out[6:10] != 0).any()

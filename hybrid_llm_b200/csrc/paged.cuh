@@ -75,11 +75,26 @@ __device__ __forceinline__ float fast_rcp(float x) {
   return y;
 }
 
-// tanh x = 1 - 2 / (1 + e^2x): absolute error below 2^-21 (one exp2 and one
-// reciprocal of the special-function unit; the tanh instruction's 2^-11 would
-// move a score capped at 50 by 0.02, a probability by 2 %).
-__device__ __forceinline__ float tanh_exp(float x) {
-  return 1.f - 2.f * fast_rcp(1.f + fast_exp2(x * (2.f * kLog2e)));
+// tanh x ~ x P(x^2) for |x| < 1: minimax fit of the RELATIVE error, 5.9e-7
+// (7.0e-7 with fp32 rounding), so that a score far below the cap keeps its digits
+// however large the cap is.
+constexpr double kTanh0 = 0.9999994135992633, kTanh1 = -0.3332904237853046,
+                 kTanh2 = 0.1328143388070316, kTanh3 = -0.05160567400105457,
+                 kTanh4 = 0.016743115062558066, kTanh5 = -0.003067060326103062;
+
+// tanh x: that, and from 1 on 1 - 2 / (1 + e^2x), whose ABSOLUTE error of 2^-22
+// (one exp2 and one reciprocal of the special-function unit) would be
+// multiplied by the cap for small x (0.012 of a score at a cap of 1e5); the tanh
+// instruction's 2^-11 would move a score capped at 50 by 0.02, a probability by 2 %.
+__device__ __forceinline__ float tanh_of(float x) {
+  const float z = x * x;
+  float p = fmaf(z, static_cast<float>(kTanh5), static_cast<float>(kTanh4));
+  p = fmaf(z, p, static_cast<float>(kTanh3));
+  p = fmaf(z, p, static_cast<float>(kTanh2));
+  p = fmaf(z, p, static_cast<float>(kTanh1));
+  p = fmaf(z, p, static_cast<float>(kTanh0));
+  const float far = 1.f - 2.f * fast_rcp(1.f + fast_exp2(x * (2.f * kLog2e)));
+  return fabsf(x) < 1.f ? p * x : far;  // far: a NaN too
 }
 
 // natural log-sum-exp from the base-2 maximum and the weight sum (0: no key)
@@ -117,24 +132,26 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return d;
 }
 
-// tanh of half of each value, |y| < 2: an odd polynomial, minimax fit of the
-// absolute error (2.2e-7).  The factor 1/2 makes "out of range" one bit of the
-// argument (2^1 and above, infinities and NaN have bit 30 set).
+// tanh of half of each value, |y| < 2, by the same with the factor 1/2 in the
+// coefficients: "out of range" is one bit of the argument (2^1 and above,
+// infinities and NaN have bit 30 set).
 __device__ __forceinline__ uint64_t tanh_half_poly2(uint64_t y) {
   const uint64_t z = mul2(y, y);
   auto c = [](double v) { return make2(static_cast<float>(v), static_cast<float>(v)); };
-  uint64_t p = fma2(z, c(-0.0028382681775838137 / 2048), c(0.016108887270092964 / 512));
-  p = fma2(z, p, c(-0.05096546933054924 / 128));
-  p = fma2(z, p, c(0.1325313001871109 / 32));
-  p = fma2(z, p, c(-0.3332393765449524 / 8));
-  p = fma2(z, p, c(0.9999968856 / 2));
+  uint64_t p = fma2(z, c(kTanh5 / 2048), c(kTanh4 / 512));
+  p = fma2(z, p, c(kTanh3 / 128));
+  p = fma2(z, p, c(kTanh2 / 32));
+  p = fma2(z, p, c(kTanh1 / 8));
+  p = fma2(z, p, c(kTanh0 / 2));
   return mul2(p, y);
 }
 
-// tanh of half of each value, any y: with x = y / 2 clamped to 7, x P(x^2) /
-// Q(x^2), minimax fit of the absolute error (9e-7; 1.7e-6 where clamped); one
-// reciprocal serves both: a/b and c/d are a d / (b d) and c b / (b d), Q in [1, 70].
+// tanh of half of each value, any y: that within its range, and beyond it, with
+// x = y / 2 clamped to 7, x P(x^2) / Q(x^2), minimax fit of the absolute error
+// (1.1e-6 with fp32 rounding; 1.7e-6 where clamped); one reciprocal serves both:
+// a/b and c/d are a d / (b d) and c b / (b d), Q in [1, 91].
 __device__ __forceinline__ uint64_t tanh_half2(uint64_t y) {
+  const float2 near = split2(tanh_half_poly2(y));
   const float2 c = split2(y);
   // the clamp drops a NaN, which would reach the other value by the reciprocal
   const float lo = fminf(fmaxf(0.5f * c.x, -7.f), 7.f), hi = fminf(fmaxf(0.5f * c.y, -7.f), 7.f);
@@ -150,7 +167,8 @@ __device__ __forceinline__ uint64_t tanh_half2(uint64_t y) {
   const float2 d = split2(q);
   const float r = fast_rcp(d.x * d.y);
   const float2 t = split2(mul2(mul2(p, make2(d.y, d.x)), make2(r, r)));
-  return make2(c.x == c.x ? t.x : c.x, c.y == c.y ? t.y : c.y);
+  auto of = [](float v, float in, float out) { return fabsf(v) < 2.f ? in : v == v ? out : v; };
+  return make2(of(c.x, near.x, t.x), of(c.y, near.y, t.y));
 }
 
 inline int page_shift_of(int page_size) {

@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) paged_decode_kernel(D
       for (int e = 0; e < 4; ++e) {
         const int key = key0 + 8 * n + c0 + (e & 1);
         float x = s[n][e];
-        if (a.softcap > 0.f) x = cap * tanh_exp(x * cap_in);
+        if (a.softcap > 0.f) x = cap * tanh_of(x * cap_in);
         else x *= sc;
         if (a.slopes) x = fmaf(-slope[e >> 1], pf - static_cast<float>(key), x);
         x = key >= cu.lo && key < cu.len ? x : -INFINITY;

@@ -706,8 +706,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
           if (__builtin_expect(edge, 0)) {  // what is not visible chooses no path below
             keep(sr, lo_c, hi_c, 0u);
           }
-          // cap tanh(s / cap): the short form in rows with |s| < cap, which one
-          // bit of 2 s / cap tells
+          // cap tanh(s / cap): the short form where every row of the warp has
+          // |s| < cap, which one bit of 2 s / cap tells; the long one gives such
+          // scores the same result
           const float in = 2.f * a.scale / a.softcap;
           const uint64_t in2 = make2(in, in);
           uint32_t big = 0u;
@@ -719,10 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
           const bool wide = live && (big & 0x40000000u);
           if (__builtin_expect(__any_sync(0xffffffffu, wide), 0)) {
 #pragma unroll
-            for (int e = 0; e < 128; e += 2) {
-              const uint64_t y = pair(sr, e);
-              set_pair(sr, e, wide ? tanh_half2(y) : tanh_half_poly2(y));
-            }
+            for (int e = 0; e < 128; e += 2) set_pair(sr, e, tanh_half2(pair(sr, e)));
           } else {
 #pragma unroll
             for (int e = 0; e < 128; e += 2) set_pair(sr, e, tanh_half_poly2(pair(sr, e)));

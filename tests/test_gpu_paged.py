@@ -796,3 +796,42 @@ def test_prefill_window_where_tokens_have_no_position(cuda, window):
     kernels.check_device_status()
     _check(out, lse, cache, q, cu, torch.bfloat16, window=window)
     assert (out[:6] == 0).all() and (out[6:10] != 0).any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("softcap,size", [(0.5, 8.0), (3.0, 12.0), (1000.0, 2.0), (1e5, 8.0)])
+@pytest.mark.parametrize("dim,page,width", [(64, 16, 0), (128, 64, 900)])
+def test_caps_far_from_the_scores(cuda, dtype, softcap, size, dim, page, width):
+    """Scores past the cap (saturated beside unsaturated ones in a warp) and caps far
+    above them, by both operators; whole and cut units.  `size` times the scores of
+    the file's tolerance, so `size` times its score terms; tanh is off by 2^-19 of
+    itself at most, below that."""
+    from hybrid_llm_b200 import kernels
+    dt = DT[dtype]
+    new, context = [150, 3, 40], [0, 200 + width, 90]
+    lengths = [a + b for a, b in zip(new, context)]
+    cache = Cache(lengths, 2, dim, page, dt, seed=66 + dim)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    g = torch.Generator().manual_seed(10)
+    q = torch.randn(cu[-1], 6, dim, generator=g)
+    q[::3] *= size  # a third of the rows
+    q = q.to(dt).cuda()
+    last = [int(x) - 1 for x in cu[1:]]
+    u, score = U[dt], size * 2.0 ** -13
+    for call, rows, begin in (
+            (lambda q, **o: kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld,
+                                                  torch.from_numpy(cu.astype(np.int32)).cuda(), **o),
+             list(range(cu[-1])), cu),
+            (lambda q, **o: kernels.paged_decode(q, cache.kd, cache.vd, cache.td, cache.ld, **o),
+             last, np.arange(4))):
+        qr = q[rows].contiguous()
+        lse = torch.empty(len(rows), 6, device="cuda")
+        out = call(qr, softcap=softcap, lse=lse)
+        kernels.check_device_status()
+        ref, mag, l_ref = paged.attention(_np(qr), cache.k_ref, cache.v_ref, cache.table, lengths,
+                                          begin, scale=dim ** -0.5, softcap=softcap)
+        tol = u * np.abs(ref) + (u + 2 * score) * mag
+        if dt is torch.float16:
+            tol = tol + max(lengths) * 2.0 ** -25 * np.abs(cache.v_ref).max()
+        assert (np.abs(_np(out) - ref) <= tol).all()
+        assert (np.abs(_np(lse) - l_ref) <= score + 2.0 ** -20 * np.abs(l_ref)).all()

@@ -103,7 +103,8 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(AppendArgs a,
   }
   dst += 8 * l;
   const float* const norm = kind == 0 ? a.q_norm : a.k_norm;
-  const bool copy = kind == 2 || (norm == nullptr && a.half == 0);
+  // a query without a position is zero whatever norm and angle would make of it
+  const bool copy = kind == 2 || pos < 0 || (norm == nullptr && a.half == 0);
 
   // x'_k = r (x_k u_k + y_k v_k), y the other member of the pair and r the
   // inverse RMS: u = weight cos, v = -+ the other's weight sin, the same for
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(AppendArgs a,
     const int h = h0 + i * kHeads;
     if (part * (kRounds * kHeads) + i * kHeads >= heads) break;
     uint4 o = raw[i];
-    if (pos < 0) o = make_uint4(0, 0, 0, 0);  // its query is zero
+    if (pos < 0) o = make_uint4(0, 0, 0, 0);
     if (!copy) {
       uint4 p = o;  // the pairs' other members
       if (!a.interleaved && a.half > 0) {

@@ -835,3 +835,27 @@ def test_caps_far_from_the_scores(cuda, dtype, softcap, size, dim, page, width):
             tol = tol + max(lengths) * 2.0 ** -25 * np.abs(cache.v_ref).max()
         assert (np.abs(_np(out) - ref) <= tol).all()
         assert (np.abs(_np(lse) - l_ref) <= score + 2.0 ** -20 * np.abs(l_ref)).all()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_append_idle_slots_are_zero(cuda, packed):
+    """A token without a position: its query is zero with eps = 0, with a weight that
+    is not finite and with query rows that are not; nothing is stored for it."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([0, 5, 0], 1, 64, 16, torch.bfloat16, seed=67)
+    x = torch.randn(3, 4, 64, device="cuda").bfloat16()
+    x[0, 0], x[2, 1, 3] = 0, float("nan")
+    w = torch.ones(64, device="cuda")
+    w[7] = float("inf")
+    before = cache.kd.clone(), cache.vd.clone()
+    cu = torch.arange(4, dtype=torch.int32, device="cuda") if packed else None
+    inv = torch.tensor([float("inf")] * 8 + [1.0] * 8, device="cuda")
+    q = kernels.paged_append(x[:, :2], x[:, 2:3], x[:, 3:], cache.kd, cache.vd, cache.td, cache.ld,
+                             cu_q=cu, eps=0.0, q_norm=w, inv_freq=inv)
+    kernels.check_device_status()
+    assert (q[0] == 0).all() and (q[2] == 0).all() and not q[1].isfinite().all()
+    p = int(cache.table[1, 0])
+    assert torch.equal(cache.vd[p, :, 4], x[1, 3:])
+    for was, now in zip(before, (cache.kd, cache.vd)):
+        was[p, :, 4] = now[p, :, 4]
+        assert torch.equal(was.view(torch.int16), now.view(torch.int16))

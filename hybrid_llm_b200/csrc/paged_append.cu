@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(AppendArgs a,
   }
   int b = tok, pos;
   if (a.cu_q != nullptr) {
-    const int end = a.cu_q[a.pool.batch];
+    const int begin = a.cu_q[0], end = a.cu_q[a.pool.batch];
     // the last b with cu_q[b] <= tok, 32 candidates at a time
     b = 0;
     for (int n = a.pool.batch; n > 1;) {
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(AppendArgs a,
       b += skip;
       n = min(step, n - skip);
     }
-    if (tok >= end) return;  // rows behind the last sequence
+    if (tok < begin || tok >= end) return;  // rows of no sequence
     pos = a.pool.lengths[b] - a.cu_q[b + 1] + tok;
   } else {
     pos = a.pool.lengths[b] - 1;

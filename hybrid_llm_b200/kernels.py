@@ -1210,8 +1210,8 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     stored in k_pages / v_pages [pages, Hkv, page_size, Dh] (any page, head and
     row strides) at block_table [B, W] int32.  lengths [B] int32 count the new
     tokens too: tokens cu_q[b] .. cu_q[b+1) (int32 [B+1]; None: one per
-    sequence) are the last positions of sequence b.  Rows behind cu_q[B] are
-    left alone; a token at a negative position (a slot of length 0) is not
+    sequence) are the last positions of sequence b.  Rows before cu_q[0] and
+    behind cu_q[B] are left alone; a token at a negative position (a slot of length 0) is not
     stored and its query is zero.  q_out may be q."""
     return _paged_call(_APPEND, q, k, v, k_pages, v_pages, block_table, lengths, cu_q, None, None,
                        q_norm, k_norm, inv_freq, q_out, None, _paged_status(q), None, 0.0,
@@ -1246,8 +1246,8 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     q [N, Hq, Dh] packed by cu_q; scores as in paged_decode.  A token at
     position i sees the keys j <= i of its own sequence with i - j < window
     (window > 0) or, instead of a window, also those j < prefix[b] (int32 [B]:
-    a bidirectional prefix).  Rows that see no key give zeros; rows behind
-    cu_q[B] are left alone.  lse: fp32 [N, Hq]."""
+    a bidirectional prefix).  Rows that see no key give zeros; rows before
+    cu_q[0] and behind cu_q[B] are left alone.  lse: fp32 [N, Hq]."""
     return _paged_call(_PREFILL, q, None, None, k_pages, v_pages, block_table, lengths, cu_q,
                        prefix, slopes, None, None, None, out, lse, _paged_status(q), scale,
                        softcap, 0.0, window, False)

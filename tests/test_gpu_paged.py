@@ -859,3 +859,35 @@ def test_append_idle_slots_are_zero(cuda, packed):
     for was, now in zip(before, (cache.kd, cache.vd)):
         was[p, :, 4] = now[p, :, 4]
         assert torch.equal(was.view(torch.int16), now.view(torch.int16))
+
+
+def test_packing_that_begins_behind_row_0(cuda):
+    """cu_q of some sequences of a larger packed batch: the rows before cu_q[0] belong
+    to none of them, in append as in prefill."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([40, 20], 2, 64, 16, torch.bfloat16, seed=68)
+    cu = [7, 12, 15]
+    cud = torch.tensor([0, 3, *cu, 18], dtype=torch.int32, device="cuda")[2:5]
+    x = torch.randn(18, 8, 64, device="cuda").bfloat16()
+    before = cache.kd.clone(), cache.vd.clone()
+    q = torch.full((18, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    kernels.paged_append(x[:, :4], x[:, 4:6], x[:, 6:], cache.kd, cache.vd, cache.td, cache.ld,
+                         cu_q=cud, q_out=q)
+    kernels.check_device_status()
+    assert (q[:7] == 7).all() and (q[15:] == 7).all() and torch.equal(q[7:15], x[7:15, :4])
+    stored = torch.zeros(cache.pages, 16, dtype=torch.bool, device="cuda")
+    for b in range(2):
+        for i in range(cu[b], cu[b + 1]):
+            at = int(cache.lengths[b]) - cu[b + 1] + i
+            p, r = cache.table[b, at // 16], at % 16
+            stored[int(p), r] = True
+            assert torch.equal(cache.kd[p, :, r], x[i, 4:6]) and torch.equal(cache.vd[p, :, r], x[i, 6:])
+            cache.k_ref[p, :, r], cache.v_ref[p, :, r] = _np(x[i, 4:6]), _np(x[i, 6:])
+    keep = ~stored[:, None, :, None].expand(cache.k.shape)
+    for was, now in zip(before, (cache.kd, cache.vd)):
+        assert torch.equal(was[keep].view(torch.int16), now[keep].view(torch.int16))
+    out = torch.full((18, 4, 64), 9.0, dtype=torch.bfloat16, device="cuda")
+    kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld, cud, out=out)
+    kernels.check_device_status()
+    assert (out[:7] == 9).all() and (out[15:] == 9).all()
+    _check(out[7:], None, cache, q[7:15], np.asarray(cu) - 7, torch.bfloat16)

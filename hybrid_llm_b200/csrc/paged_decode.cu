@@ -269,7 +269,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) paged_decode_kernel(D
         Elem<T>::mma(s[2 * n2 + 1], qf[ks], bk[2], bk[3]);
       }
     const int key0 = (cu.first + cu.tile) * KT;
-    const float pf = static_cast<float>(cu.len - 1);
+    // distance of the lane's first key: formed in whole numbers, positions pass 2^24
+    const float d0 = static_cast<float>(cu.len - 1 - key0 - c0);
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int n = 0; n < KT / 8; ++n)
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) paged_decode_kernel(D
         float x = s[n][e];
         if (a.softcap > 0.f) x = cap * tanh_of(x * cap_in);
         else x *= sc;
-        if (a.slopes) x = fmaf(-slope[e >> 1], pf - static_cast<float>(key), x);
+        if (a.slopes) x = fmaf(-slope[e >> 1], d0 - static_cast<float>(8 * n + (e & 1)), x);
         x = key >= cu.lo && key < cu.len ? x : -INFINITY;
         s[n][e] = x;
         top[e >> 1] = fmaxf(top[e >> 1], x);

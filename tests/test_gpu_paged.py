@@ -891,3 +891,31 @@ def test_packing_that_begins_behind_row_0(cuda):
     kernels.check_device_status()
     assert (out[:7] == 9).all() and (out[15:] == 9).all()
     _check(out[7:], None, cache, q[7:15], np.asarray(cu) - 7, torch.bfloat16)
+
+
+@pytest.mark.parametrize("far", [2 ** 25 + 128, 2 ** 30 - 4096])
+def test_bias_and_window_at_far_positions(cuda, far):
+    """Positions that fp32 does not hold: the same last keys as a short sequence's, seen
+    through a window with a distance bias, behind a table of any other pages."""
+    from hybrid_llm_b200 import kernels
+    page, dim = 256, 64
+    cache = Cache([700], 1, dim, page, torch.bfloat16, seed=69, pad=0)
+    g = torch.Generator().manual_seed(11)
+    q = torch.randn(9, 4, dim, generator=g).bfloat16().cuda()
+    slopes = torch.tensor([0.9, 0.3, 0.05, -0.01], device="cuda")
+    first = far // page  # pages before the short sequence's
+    table = torch.full((1, first + cache.td.shape[1]), -1, dtype=torch.int32, device="cuda")
+    table[:, first:] = cache.td
+    lengths = cache.ld + first * page
+    cu = np.asarray([0, 9])
+    lse = torch.empty(9, 4, device="cuda")
+    out = kernels.paged_prefill(q, cache.kd, cache.vd, table, lengths,
+                                torch.tensor([0, 9], dtype=torch.int32, device="cuda"), window=300,
+                                slopes=slopes, lse=lse)
+    kernels.check_device_status()
+    _check(out, lse, cache, q, cu, torch.bfloat16, window=300, slopes=_np(slopes))
+    lse = torch.empty(1, 4, device="cuda")
+    out = kernels.paged_decode(q[8:], cache.kd, cache.vd, table, lengths, window=300, slopes=slopes,
+                               lse=lse)
+    kernels.check_device_status()
+    _check(out, lse, cache, q[8:], np.asarray([0, 1]), torch.bfloat16, window=300, slopes=_np(slopes))

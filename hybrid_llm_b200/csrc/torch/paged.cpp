@@ -159,8 +159,11 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t count) {
       if (!(softcap >= 0.0) || window < 0) refuse("softcap and window must be >= 0 (0: none)");
       if (!scaled) scale = 1.0 / std::sqrt(static_cast<double>(a.head_dim));
       a.scale = static_cast<float>(scale), a.softcap = static_cast<float>(softcap);
-      if (!(a.scale > 0.f) || std::isinf(a.scale) || std::isinf(a.softcap))
-        refuse("scale must be positive, scale and softcap finite");
+      if (!std::isnormal(a.scale) || a.scale < 0.f || !std::isnormal(a.scale * 1.5f))
+        refuse("scale must be positive and finite");
+      if (softcap > 0.0 && (!std::isnormal(a.softcap * 1.5f) || !std::isnormal(a.scale / a.softcap) ||
+                            !std::isnormal(2.f * a.scale / a.softcap)))
+        refuse("softcap, or scale / softcap, is beyond what fp32 holds");
       a.window = whole(window, "window");
       a.slopes = vector<float>(t[9], "slopes", at::kFloat, a.q_heads);
       a.prefix = vector<int32_t>(t[8], "prefix", at::kInt, a.batch);

@@ -840,7 +840,8 @@ int32_t llmyb_paged_append(const llmyb_paged_args* args, void* stream);
 
 /* One token per sequence (n_tokens == batch; row b of q and out has position
  * lengths[b] - 1): out = softmax(s) v over its visible keys, s = scale q.k
- * (scale > 0), then softcap * tanh(s / softcap) if softcap > 0, then
+ * (scale > 0), then softcap * tanh(s / softcap) if softcap > 0 (scale, softcap
+ * and scale / softcap normal numbers of fp32, twice over: LLMYB_EINVAL), then
  * - slopes[h] * distance if slopes; window > 0: distance < window.  A sequence
  * of length 0 gives zeros.  lse: natural log of the sum of exp(s), -inf where
  * no key is visible.  scratch: scratch_bytes of the current device, not shared

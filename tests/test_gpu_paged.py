@@ -919,3 +919,18 @@ def test_bias_and_window_at_far_positions(cuda, far):
                                lse=lse)
     kernels.check_device_status()
     _check(out, lse, cache, q[8:], np.asarray([0, 1]), torch.bfloat16, window=300, slopes=_np(slopes))
+
+
+def test_scores_that_fp32_does_not_hold_are_refused(cuda):
+    """A cap that is 0 in fp32 is not taken for none; factors beyond fp32 are refused."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([40], 2, 64, 16, torch.bfloat16, seed=50)
+    q = torch.randn(1, 4, 64, device="cuda").bfloat16()
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    ok = (cache.kd, cache.vd, cache.td, cache.ld)
+    for f, tail in ((kernels.paged_decode, ()), (kernels.paged_prefill, (cu,))):
+        for over in (dict(softcap=1e-50), dict(softcap=1e-39), dict(softcap=1e38),
+                     dict(softcap=float("inf")), dict(softcap=1e39), dict(scale=1e-45),
+                     dict(scale=3e38), dict(scale=4.0, softcap=1e-38), dict(scale=1e-30, softcap=1e9)):
+            with pytest.raises(ValueError):
+                f(q, *ok, *tail, **over)

@@ -235,3 +235,13 @@ def test_advance_refuses_what_has_no_page():
     c.advance([22, 13, 0])
     c.reserve([1, 1, 0])
     assert [len(r) for r in _rows(c)] == [3, 2, 0]
+
+
+@pytest.mark.parametrize("entry", [DECODE, PREFILL])
+def test_scores_that_fp32_does_not_hold_are_refused(entry):
+    """A scale or a cap whose factors overflow or vanish: every score would be 0 or NaN."""
+    inf = float("inf")
+    for over in (dict(scale=inf), dict(scale=3e38), dict(scale=1e-40), dict(softcap=inf),
+                 dict(softcap=3e38), dict(softcap=1e-39), dict(softcap=1e38), dict(scale=4.0, softcap=1e-38),
+                 dict(scale=1e-30, softcap=1e9)):
+        assert _status(entry, _args(**over)) == _native.LLMYB_EINVAL, over

@@ -60,6 +60,25 @@ void* rows(const at::Tensor* t, const char* name, int64_t tokens, int64_t heads,
   return t->data_ptr();
 }
 
+// what is written has one place per element: by stride, every dimension steps
+// over all that the smaller ones span
+void apart(const at::Tensor& t, const char* name) {
+  int64_t span = 0, last = -1;
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    int64_t next = -1;  // the smallest stride not yet seen
+    for (int64_t d = 0; d < t.dim(); ++d) {
+      if (t.size(d) < 2) continue;
+      if (t.stride(d) > last && (next < 0 || t.stride(d) < t.stride(next))) next = d;
+      for (int64_t e = 0; e < d; ++e)
+        if (t.size(e) > 1 && t.stride(e) == t.stride(d)) refuse(text(name, " overlaps itself"));
+    }
+    if (next < 0) return;
+    last = t.stride(next);
+    if (last <= span) refuse(text(name, " overlaps itself"));
+    span += last * (t.size(next) - 1);
+  }
+}
+
 template <typename T>
 T* vector(const at::Tensor* t, const char* name, at::ScalarType type, int64_t n) {
   if (t == nullptr) return nullptr;
@@ -140,6 +159,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t count) {
                               : "without cu_q there is one token per sequence of block_table");
     int64_t scratch_bytes = 0;
     if (kind == kAppend) {
+      apart(kp, "k_pages and v_pages");  // alike
       a.k = rows(t[1], "k", a.n_tokens, a.kv_heads, a.head_dim, type, a.k_token_stride, a.k_head_stride);
       a.v = rows(t[2], "v", a.n_tokens, a.kv_heads, a.head_dim, type, a.v_token_stride, a.v_head_stride);
       const int64_t half = t[12] ? t[12]->numel() : 0;
@@ -184,6 +204,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t count) {
     at::Tensor out;
     if (t[13]) {
       out = *t[13];
+      apart(out, names[13]);
     } else {
       out = at::empty({a.n_tokens, a.q_heads, a.head_dim}, q.options());
     }

@@ -934,3 +934,34 @@ def test_scores_that_fp32_does_not_hold_are_refused(cuda):
                      dict(scale=3e38), dict(scale=4.0, softcap=1e-38), dict(scale=1e-30, softcap=1e9)):
             with pytest.raises(ValueError):
                 f(q, *ok, *tail, **over)
+
+
+def test_outputs_that_overlap_themselves_are_refused(cuda):
+    """Expanded or overlapping outputs and pools have no place of their own for every
+    element; any order of the dimensions, and gaps, are fine."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([40, 9], 2, 64, 16, torch.bfloat16, seed=50)
+    q = torch.randn(2, 4, 64, device="cuda").bfloat16()
+    kv = torch.randn(2, 2, 64, device="cuda").bfloat16()
+    cu = torch.arange(3, dtype=torch.int32, device="cuda")
+    at = (cache.td, cache.ld)
+    pages = (cache.kd, cache.vd)
+    flat = torch.zeros(4096, dtype=torch.bfloat16, device="cuda")
+    for strides in ((0, 64, 1), (256, 0, 1), (64, 64, 1), (256, 32, 1), (192, 64, 1), (8, 64, 1)):
+        out = flat.as_strided((2, 4, 64), strides)
+        for call in (lambda: kernels.paged_decode(q, *pages, *at, out=out),
+                     lambda: kernels.paged_prefill(q, *pages, *at, cu, out=out),
+                     lambda: kernels.paged_append(q, kv, kv, *pages, *at, q_out=out)):
+            with pytest.raises(ValueError, match="overlaps itself"):
+                call()
+    pool = cache.kd[:, :1].expand(-1, 2, -1, -1)
+    with pytest.raises(ValueError, match="overlaps itself"):
+        kernels.paged_append(q, kv, kv, pool, pool, *at)
+    want = kernels.paged_decode(q, *pages, *at)
+    for strides in ((256, 64, 1), (64, 128, 1), (72, 144, 1), (1024, 128, 1)):
+        out = flat.as_strided((2, 4, 64), strides)
+        assert torch.equal(kernels.paged_decode(q, *pages, *at, out=out), want)
+        assert torch.equal(out, want)
+    one = flat.as_strided((1, 4, 64), (0, 64, 1))
+    assert torch.equal(kernels.paged_decode(q[:1], *pages, cache.td[:1], cache.ld[:1], out=one), want[:1])
+    kernels.check_device_status()

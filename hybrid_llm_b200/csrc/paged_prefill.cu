@@ -354,15 +354,25 @@ struct Units {
 // A wait that polls: the suspending wait of sm100.cuh wakes up to a
 // microsecond late, which the chain S -> P -> O pays twice per block
 // (prefill of 8192 tokens: 769 us with it, 614 us polling).  Bounded like it.
-// Every lane waits for itself: a phase that one lane has seen complete stays so
-// until its warp goes on, so the lanes agree without a vote (which cost 4 %);
-// after another role's timeout a late completion counts as none.
+// By a whole warp, whose lanes leave with one answer (what follows is for
+// converged warps, after a timeout too): every lane polls for itself and one
+// vote tells whether all have seen the phase complete.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int32_t* status,
                                      volatile int* abort_flag) {
-  for (int i = 0; i < 4096; ++i)
-    if (sm100::mbar_try_wait(bar, parity)) return true;
-  return sm100::mbar_wait(bar, parity, status, abort_flag) &&
-         (abort_flag == nullptr || !*abort_flag);
+  for (uint64_t t0 = 0;;) {
+    bool ok = false;
+    for (int i = 0; i < 4096 && !ok; ++i) ok = sm100::mbar_try_wait(bar, parity);
+    if (__all_sync(0xffffffffu, ok)) return true;
+    bool stop = abort_flag != nullptr && *abort_flag;
+    const uint64_t now = globaltimer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) {
+      report_status(status, LLMYB_ETIMEOUT);
+      if (abort_flag != nullptr) *abort_flag = 1;
+      stop = true;
+    }
+    if (__any_sync(0xffffffffu, stop)) return false;
+  }
 }
 
 // elements e and e + 1 of a row of scores

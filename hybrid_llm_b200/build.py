@@ -4,11 +4,13 @@
 nvcc for ``sm_100a`` and links ``hybrid_llm_b200/lib/libllmyb.so``.  Objects
 are cached under ``_build/`` and rebuilt only when a source or header is newer.
 ``csrc/torch/*.cpp`` becomes ``hybrid_llm_b200/lib/llmyb_torch.so``, a Python
-module that takes torch tensors and calls the library (g++, torch's headers).
+module that takes torch tensors and calls the library (g++, torch's headers;
+built again when torch or Python change, left out where they are missing).
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -54,6 +56,18 @@ def _compile(src: Path, obj: Path, verbose: bool) -> None:
         print(res.stdout + res.stderr, file=sys.stderr)
 
 
+def _torch_missing() -> str:
+    """What the tensor-level module cannot be built without and is not there ("": nothing)."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        return "torch"
+    if not (Path(spec.submodule_search_locations[0]) / "include/ATen/ATen.h").exists():
+        return "torch's headers"
+    if not (Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
+        return "Python's headers"
+    return "" if shutil.which("g++") else "g++"
+
+
 def _torch_module(verbose: bool) -> None:
     """The tensor-level module; torch itself is not imported."""
     torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
@@ -71,6 +85,26 @@ def _torch_module(verbose: bool) -> None:
     if verbose and (res.stdout or res.stderr):
         print(res.stdout + res.stderr, file=sys.stderr)
     os.replace(tmp, TORCH_LIB)
+
+
+def _build_torch_module(force: bool, verbose: bool) -> None:
+    """Builds the tensor-level module where it is out of date.  The native library
+    and engine do without it: where it cannot be built it is left out (a module
+    of older sources would pass another argument block), and loading it raises."""
+    stamp = BUILD / "llmyb_torch.stamp"
+    missing = _torch_missing()
+    want = missing or f"torch {importlib.metadata.version('torch')}, python {sys.version}"
+    inputs = [*(CSRC / "torch").glob("*.cpp"), *(PKG.parent / "include").glob("*.h")]
+    if (not force and TORCH_LIB.exists() and stamp.exists() and stamp.read_text() == want
+            and TORCH_LIB.stat().st_mtime >= max(f.stat().st_mtime for f in inputs)):
+        return
+    if missing:
+        TORCH_LIB.unlink(missing_ok=True)
+        print(f"{TORCH_LIB.name} is not built: {missing} not found (the paged cache's Python calls "
+              "need it)", file=sys.stderr)
+        return
+    _torch_module(verbose)
+    stamp.write_text(want)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -98,10 +132,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
-    made = TORCH_LIB.stat().st_mtime if TORCH_LIB.exists() and not force else 0.0
-    inputs = [*(CSRC / "torch").glob("*.cpp"), *(PKG.parent / "include").glob("*.h")]
-    if made < max(f.stat().st_mtime for f in inputs):
-        _torch_module(verbose)
+    _build_torch_module(force, verbose)
     return LIB
 
 

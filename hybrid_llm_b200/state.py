@@ -267,8 +267,12 @@ class PagedKVCache:
         self._length = length
 
     def release(self, rows) -> None:
-        """Gives the pages of the rows back; their lengths are 0."""
-        for b in {int(r) for r in rows}:
+        """Gives the pages of the rows back; their lengths are 0.  Raises and changes
+        nothing where a row is none of the batch's."""
+        rows = {int(r) for r in rows}
+        if any(r < 0 or r >= self.batch for r in rows):
+            raise ValueError(f"rows 0 .. {self.batch - 1} can be released")
+        for b in rows:
             self._free += reversed(self._held[b])
             self._held[b], self._length[b] = [], 0
             self.block_table[b].fill_(-1)

@@ -245,3 +245,16 @@ def test_scores_that_fp32_does_not_hold_are_refused(entry):
                  dict(softcap=3e38), dict(softcap=1e-39), dict(softcap=1e38), dict(scale=4.0, softcap=1e-38),
                  dict(scale=1e-30, softcap=1e9)):
         assert _status(entry, _args(**over)) == _native.LLMYB_EINVAL, over
+
+
+@pytest.mark.parametrize("rows", [[0, 3], [-1], [1, -3], [99]])
+def test_release_of_rows_that_are_none(rows):
+    c = _cache()
+    c.extend([20, 5, 16])
+    state = _rows(c), c.lengths.tolist(), c.free_pages
+    with pytest.raises(ValueError, match="released"):
+        c.release(rows)
+    assert (_rows(c), c.lengths.tolist(), c.free_pages) == state
+    c.release([])
+    c.release([2, 2, 0])
+    assert c.lengths.tolist() == [0, 5, 0] and c.free_pages == 7

@@ -33,12 +33,19 @@ struct PagedPool {
   }
 };
 
-// 16-bit element types: pack two fp32 values, unpack two, 1.0 of the type.
+// 16-bit element types: pack two fp32 values, unpack two.  Softmax weights are
+// rounded to the type for the second product, in which fp16 holds nothing below
+// 2^-25: there the largest weight is 2^kDecodeUp, or in the prompt kernel
+// 2^kPrefillUp, which needs the rest for maxima that rise later, so that the many
+// small weights of a long cache are kept (with a largest weight of 1, 40,000 keys
+// 25 bits below the best one vanished from the output, 0.1 % of it, but not from
+// the weights' sum).  bf16 has the exponents of fp32.
 template <typename T>
 struct Elem;
 
 template <>
 struct Elem<__nv_bfloat16> {
+  static constexpr float kDecodeUp = 0.f, kPrefillUp = 0.f, kMostWeight = 16384.f;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
   static __device__ __forceinline__ float2 unpack(uint32_t v) { return unpack_bf16x2(v); }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -53,6 +60,8 @@ struct Elem<__nv_bfloat16> {
 
 template <>
 struct Elem<__half> {
+  static constexpr float kDecodeUp = 12.f, kPrefillUp = 4.f;
+  static constexpr float kMostWeight = 57344.f;  // below the type's largest, 65504
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     __half2 p = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&p);

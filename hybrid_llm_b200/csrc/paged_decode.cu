@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) paged_decode_kernel(D
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2)) - Elem<T>::kDecodeUp;
     }
     if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
       float f[2];

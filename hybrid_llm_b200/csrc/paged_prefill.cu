@@ -756,7 +756,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
         }
         if (__builtin_expect(edge, 0)) keep(sr, lo_c, hi_c, 0xff800000u);  // -inf
         // m of the rows that ask for it (and of no other: a row's result does not
-        // depend on its neighbours) to the block's maximum, l and O rescaled
+        // depend on its neighbours) to the block's maximum (less kPrefillUp), l and
+        // O rescaled
         auto raise = [&](bool ask) {
           float mx[4];
 #pragma unroll
@@ -768,7 +769,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
               mx[k] = max3(mx[k], __uint_as_float(sr[e + 2 * k]), __uint_as_float(sr[e + 2 * k + 1]));
           mx[0] = max3(mx[0], __uint_as_float(sr[124]), __uint_as_float(sr[125]));
           mx[1] = max3(mx[1], __uint_as_float(sr[126]), __uint_as_float(sr[127]));
-          const float bm = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * sc;
+          const float bm =
+              fmaf(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]), sc, -Elem<T>::kPrefillUp);
           float alpha = 1.f;
           if (ask && bm > m) {
             alpha = fast_exp2(m - bm);
@@ -810,8 +812,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
           return r.x + r.y;
         };
         // The weights take the maximum of the blocks before.  Their sum shows
-        // whether that is still near enough: below 2^14 every one is (fp16
-        // holds 2^16, sums are fp32), and the block's own maximum is never
+        // whether that is still near enough: below kMostWeight every one is
+        // (fp16 holds 65504, sums are fp32), and the block's own maximum is never
         // formed (459 us against 502 with it).  Else, a NaN among them
         // included, and at a row's first keys it is.
         if (!settled) {
@@ -820,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
           settled = __all_sync(0xffffffffu, !live || m != -INFINITY);
         }
         float sum = weights();
-        const bool far = live && !(sum <= 16384.f);
+        const bool far = live && !(sum <= Elem<T>::kMostWeight);
         if (__builtin_expect(__any_sync(0xffffffffu, far), 0)) {
           raise(far);
           sum = weights();

@@ -965,3 +965,68 @@ def test_outputs_that_overlap_themselves_are_refused(cuda):
     one = flat.as_strided((1, 4, 64), (0, 64, 1))
     assert torch.equal(kernels.paged_decode(q[:1], *pages, cache.td[:1], cache.ld[:1], out=one), want[:1])
     kernels.check_device_status()
+
+
+def test_fp16_keeps_many_small_weights(cuda):
+    """40,000 keys 25.2 bits below the best one are 0.1 % of the weights' sum.  A weight
+    is off by at most 2^-25 in units of 2^-kUp of the largest (subnormal), kUp = 12 in
+    decode and 4 in prefill: n 2^-37 and n 2^-29 of max |v| beside the roundings."""
+    from hybrid_llm_b200 import kernels
+    n = 40000
+    cache = Cache([n], 1, 64, 64, torch.float16, seed=70)
+    g = torch.Generator().manual_seed(12)
+    k, v = torch.zeros(n, 64), torch.rand(n, 64, generator=g) + 0.5
+    k[0, 0], v[0] = 8.734375, 0.0            # scores 17.47 and 0
+    for t, ref, x in ((cache.kd, cache.k_ref, k), (cache.vd, cache.v_ref, v)):
+        x = x.half()
+        for i, p in enumerate(cache.table[0, :n // 64]):
+            t[int(p), 0] = x[64 * i:64 * i + 64].cuda()
+            ref[int(p), 0] = _np(x[64 * i:64 * i + 64])
+    q = torch.zeros(3, 2, 64)
+    q[:, :, 0] = 16.0
+    q = q.half().cuda()
+    cu = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    u = U[torch.float16]
+    for out, rows, up in ((kernels.paged_decode(q[2:], cache.kd, cache.vd, cache.td, cache.ld), [2], 12),
+                          (kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld, cu),
+                           [0, 1, 2], 4)):
+        kernels.check_device_status()
+        ref, mag, _ = paged.attention(_np(q[rows]), cache.k_ref, cache.v_ref, cache.table, [n],
+                                      [0, len(rows)], scale=0.125)
+        tol = u * np.abs(ref) + (u + 2 * 2.0 ** -12) * mag + n * 2.0 ** (-25 - up) * 1.5
+        assert (np.abs(_np(out) - ref) <= tol).all() and (ref > 5e-4).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("pad", [0, 40])
+@pytest.mark.parametrize("rise", [4.0, 12.0, 40.0])
+def test_maximum_that_rises_late(cuda, dtype, pad, rise):
+    """Keys are visited from the last to the first; the first ones score `rise` above the
+    rest, beyond what the weights of the block may hold; whole and cut units.  Scores
+    up to 10 + rise, so (1 + rise / 10) times the tolerance's score terms."""
+    from hybrid_llm_b200 import kernels
+    dt = DT[dtype]
+    new, context = [70, 130, 1], [330, 200, 400]
+    lengths = [a + b for a, b in zip(new, context)]
+    cache = Cache(lengths, 1, 64, 16, dt, seed=71, pad=pad)
+    for b in range(3):
+        p = int(cache.table[b, 0])
+        cache.kd[p, 0, :7, 0] = rise
+        cache.k_ref[p, 0, :7, 0] = rise
+    cu = np.concatenate([[0], np.cumsum(new)])
+    g = torch.Generator().manual_seed(13)
+    q = torch.randn(cu[-1], 2, 64, generator=g)
+    q[::2, :, 0] = 8.0                          # every other row: rise * 8 / 8
+    q = q.to(dt).cuda()
+    lse = torch.empty(cu[-1], 2, device="cuda")
+    out = kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld,
+                                torch.from_numpy(cu.astype(np.int32)).cuda(), lse=lse)
+    kernels.check_device_status()
+    ref, mag, l_ref = paged.attention(_np(q), cache.k_ref, cache.v_ref, cache.table, lengths, cu,
+                                      scale=0.125)
+    u, score = U[dt], (1 + rise / 10) * 2.0 ** -13
+    tol = u * np.abs(ref) + (u + 2 * score) * mag
+    if dt is torch.float16:
+        tol = tol + max(lengths) * 2.0 ** -25 * np.abs(cache.v_ref).max()
+    assert (np.abs(_np(out) - ref) <= tol).all()
+    assert (np.abs(_np(lse) - l_ref) <= score + 2.0 ** -20 * np.abs(l_ref)).all()

@@ -86,28 +86,6 @@ __device__ __forceinline__ float fast_rcp(float x) {
   return y;
 }
 
-// tanh x ~ x P(x^2) for |x| < 1: minimax fit of the RELATIVE error, 5.9e-7
-// (7.0e-7 with fp32 rounding), so that a score far below the cap keeps its digits
-// however large the cap is.
-constexpr double kTanh0 = 0.9999994135992633, kTanh1 = -0.3332904237853046,
-                 kTanh2 = 0.1328143388070316, kTanh3 = -0.05160567400105457,
-                 kTanh4 = 0.016743115062558066, kTanh5 = -0.003067060326103062;
-
-// tanh x: that, and from 1 on 1 - 2 / (1 + e^2x), whose ABSOLUTE error of 2^-22
-// (one exp2 and one reciprocal of the special-function unit) would be
-// multiplied by the cap for small x (0.012 of a score at a cap of 1e5); the tanh
-// instruction's 2^-11 would move a score capped at 50 by 0.02, a probability by 2 %.
-__device__ __forceinline__ float tanh_of(float x) {
-  const float z = x * x;
-  float p = fmaf(z, static_cast<float>(kTanh5), static_cast<float>(kTanh4));
-  p = fmaf(z, p, static_cast<float>(kTanh3));
-  p = fmaf(z, p, static_cast<float>(kTanh2));
-  p = fmaf(z, p, static_cast<float>(kTanh1));
-  p = fmaf(z, p, static_cast<float>(kTanh0));
-  const float far = 1.f - 2.f * fast_rcp(1.f + fast_exp2(x * (2.f * kLog2e)));
-  return fabsf(x) < 1.f ? p * x : far;  // far: a NaN too
-}
-
 // natural log-sum-exp from the base-2 maximum and the weight sum (0: no key)
 __device__ __forceinline__ float lse_of(float m, float l) {
   return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
@@ -143,7 +121,14 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return d;
 }
 
-// tanh of half of each value, |y| < 2, by the same with the factor 1/2 in the
+// tanh x ~ x P(x^2) for |x| < 1: minimax fit of the RELATIVE error, 5.9e-7
+// (7.0e-7 with fp32 rounding), so that a score far below the cap keeps its digits
+// however large the cap is.
+constexpr double kTanh0 = 0.9999994135992633, kTanh1 = -0.3332904237853046,
+                 kTanh2 = 0.1328143388070316, kTanh3 = -0.05160567400105457,
+                 kTanh4 = 0.016743115062558066, kTanh5 = -0.003067060326103062;
+
+// tanh of half of each value, |y| < 2, by that with the factor 1/2 in the
 // coefficients: "out of range" is one bit of the argument (2^1 and above,
 // infinities and NaN have bit 30 set).
 __device__ __forceinline__ uint64_t tanh_half_poly2(uint64_t y) {
@@ -157,7 +142,20 @@ __device__ __forceinline__ uint64_t tanh_half_poly2(uint64_t y) {
   return mul2(p, y);
 }
 
-// tanh of half of each value, any y: that within its range, and beyond it, with
+// The same for any y: from 2 on 1 - 2 / (1 + e^y), whose ABSOLUTE error of 2^-22
+// (one exp2 and one reciprocal of the special-function unit) would be multiplied
+// by the cap for small y (0.012 of a score at a cap of 1e5); the tanh
+// instruction's 2^-11 would move a score capped at 50 by 0.02, a probability by 2 %.
+__device__ __forceinline__ uint64_t tanh_half_exp2(uint64_t y) {
+  const float2 near = split2(tanh_half_poly2(y)), v = split2(y);
+  auto of = [](float v, float near) {
+    const float far = 1.f - 2.f * fast_rcp(1.f + fast_exp2(v * kLog2e));
+    return fabsf(v) < 2.f ? near : far;  // far: a NaN too
+  };
+  return make2(of(v.x, near.x), of(v.y, near.y));
+}
+
+// The same for any y with one special function for two values: from 2 on, with
 // x = y / 2 clamped to 7, x P(x^2) / Q(x^2), minimax fit of the absolute error
 // (1.1e-6 with fp32 rounding; 1.7e-6 where clamped); one reciprocal serves both:
 // a/b and c/d are a d / (b d) and c b / (b d), Q in [1, 91].

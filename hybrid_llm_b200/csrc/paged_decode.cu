@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) paged_decode_kernel(D
   };
   begin();
   const float sc = a.scale * kLog2e, cap = a.softcap * kLog2e;
-  const float cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+  const float cap_in = a.softcap > 0.f ? 2.f * a.scale / a.softcap : 0.f;
   bool whole_start = !a.whole && cu.tile == 0;  // this worker holds the segment's first tile
   bool first_segment = true;
   int stage = 0;
@@ -271,15 +271,42 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) paged_decode_kernel(D
     const int key0 = (cu.first + cu.tile) * KT;
     // distance of the lane's first key: formed in whole numbers, positions pass 2^24
     const float d0 = static_cast<float>(cu.len - 1 - key0 - c0);
+    if (a.softcap > 0.f) {
+      uint32_t big = 0u;  // bit 30: a score past the cap
+#pragma unroll
+      for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[n][e] *= cap_in;
+          big |= __float_as_uint(s[n][e]);
+        }
+      // they are rare; a tile without takes the short form, to the same results
+      if (__builtin_expect(__any_sync(0xffffffffu, big & 0x40000000u), 0)) {
+#pragma unroll
+        for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const float2 t = split2(tanh_half_exp2(make2(s[n][e], s[n][e + 1])));
+            s[n][e] = t.x, s[n][e + 1] = t.y;
+          }
+      } else {
+#pragma unroll
+        for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const float2 t = split2(tanh_half_poly2(make2(s[n][e], s[n][e + 1])));
+            s[n][e] = t.x, s[n][e + 1] = t.y;
+          }
+      }
+    }
+    const float to2 = a.softcap > 0.f ? cap : sc;  // to scores in base 2
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int n = 0; n < KT / 8; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = key0 + 8 * n + c0 + (e & 1);
-        float x = s[n][e];
-        if (a.softcap > 0.f) x = cap * tanh_of(x * cap_in);
-        else x *= sc;
+        float x = s[n][e] * to2;
         if (a.slopes) x = fmaf(-slope[e >> 1], d0 - static_cast<float>(8 * n + (e & 1)), x);
         x = key >= cu.lo && key < cu.len ? x : -INFINITY;
         s[n][e] = x;

@@ -48,6 +48,11 @@ struct Elem<__nv_bfloat16> {
   static constexpr float kDecodeUp = 0.f, kPrefillUp = 0.f, kMostWeight = 16384.f;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
   static __device__ __forceinline__ float2 unpack(uint32_t v) { return unpack_bf16x2(v); }
+  // acc, or NaN where v or acc is not finite
+  static __device__ __forceinline__ uint32_t probe(uint32_t v, uint32_t acc) {
+    __nv_bfloat162 r = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&v), __nv_bfloat162{}, *reinterpret_cast<__nv_bfloat162*>(&acc));
+    return *reinterpret_cast<uint32_t*>(&r);
+  }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                              uint32_t b1) {
     asm volatile(
@@ -69,6 +74,11 @@ struct Elem<__half> {
   static __device__ __forceinline__ float2 unpack(uint32_t v) {
     __half2 p = *reinterpret_cast<__half2*>(&v);
     return __half22float2(p);
+  }
+  // acc, or NaN where v or acc is not finite
+  static __device__ __forceinline__ uint32_t probe(uint32_t v, uint32_t acc) {
+    __half2 r = __hfma2(*reinterpret_cast<__half2*>(&v), __half2{}, *reinterpret_cast<__half2*>(&acc));
+    return *reinterpret_cast<uint32_t*>(&r);
   }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                              uint32_t b1) {

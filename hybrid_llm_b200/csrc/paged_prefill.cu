@@ -18,6 +18,7 @@
 //                   one ring of 128-key blocks
 //   warp 9          MMA: O_t += P_t V then S_t = Q_t K of the next block, for
 //                   t = 0, 1: one tile's products run under the other's softmax
+//   warp 10         checks the values of blocks that some row sees in part
 // S in fp32 TMEM columns; P in 16 bits over S's first columns, the A operand of
 // the second product; O in fp32 TMEM, divided by the weight sum at the end.
 //
@@ -27,11 +28,16 @@
 // range cuts leaves its unnormalised fp32 O, maxima and weight sums in scratch,
 // and a second launch joins them in a fixed order.
 //
-// Values of rows outside the sequence (behind its end, or before the window)
-// are zeroed in shared memory: they may hold anything, and a zero weight does
-// not cancel an infinity.  All waits are bounded; a timeout records
-// LLMYB_ETIMEOUT and every role unwinds.
+// Values that a row does not see meet its zero weights, which do not cancel an
+// infinity: in blocks that some row sees in part, rows outside the sequence
+// (behind its end, or before the window; they may hold anything) are zeroed in
+// shared memory, and so are values that are not finite, which are added to the
+// outputs of the rows that see them (add_not_finite).  The check runs beside the
+// block's softmax: 1.6 % of a ragged batch under a window, where every fourth
+// block is an edge.  All waits are bounded; a timeout records LLMYB_ETIMEOUT and
+// every role unwinds.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -78,6 +84,7 @@ struct CutUnit {
 
 struct PrefillArgs {
   PagedPool pool;
+  const uint16_t* v_pages;  // for add_not_finite; the rest is read by TMA
   const int32_t* cu_q;
   const int32_t* prefix;  // or null
   int32_t n_tokens, q_heads, group, tile_tokens, window;
@@ -293,12 +300,19 @@ __device__ __forceinline__ Start find_start(const PrefillArgs& a, int64_t* sums,
 // A unit, or the part of it in one CTA's range, as the roles get it.
 struct Unit {
   int blocks;         // key blocks [kb0, kb0 + blocks); -1: no more units
+  int seq, len;       // sequence and its length
   int kb0, tiles;     // tiles with tokens
   int kvh;
   int token, count;   // first token, how many
   int pos;            // position of the first token
   int prefix;
   int starts, ends;   // the part holds the unit's last keys / first keys
+  int first;          // first key that any row sees
+  int lo, hi;         // the keys that every row sees
+  int odd;            // values were left out for add_not_finite
+
+  // some row does not see all keys of the block at j0
+  __device__ __forceinline__ bool edge(int j0) const { return j0 + kRows - 1 > hi || j0 < lo; }
 };
 
 // The units of one CTA's range, in order.
@@ -337,12 +351,18 @@ struct Units {
       }
       if (s0 >= s1 && !(all == 0 && first)) continue;
       u.blocks = s1 - s0;
+      u.seq = b;
       u.kb0 = kb0 + all - s1;
       u.count = min(2 * a.tile_tokens, s.n - t0);
       u.tiles = u.count > a.tile_tokens ? 2 : 1;
       u.token = s.q0 + t0;
       u.pos = s.len - s.n + t0;
       u.prefix = s.prefix;
+      u.len = s.len;
+      u.first = lo;
+      u.lo = first_key(a, u.pos + u.count - 1);
+      u.hi = u.pos < 0 ? -1 : max(u.pos, u.prefix - 1);
+      u.odd = 0;
       u.starts = s0 == 0;
       u.ends = s1 == all;
       return true;
@@ -405,6 +425,83 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// The bits of a packed pair's values that are not finite.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return ((w & e) == e ? 0xffffu : 0u) | ((w >> 16 & e) == e ? 0xffff0000u : 0u);
+}
+
+// Values that are not finite were left out of a unit's edge blocks, as rows see
+// them that do not see their keys.  This adds them, from memory, to the stored
+// outputs of the rows that do: with any weight they make an infinity or a NaN.  By
+// a whole warp, a lane per row of the tile (dst, part: where its output is) and
+// a lane per D / 32 columns; rare, and it reads the edge blocks' values alone.
+template <typename T, int D>
+__device__ __forceinline__ void add_not_finite(const PrefillArgs& a, const Unit& u, bool live, int lo,
+                                               int hi, int64_t dst, float4* part) {
+  constexpr int kWords = D / 64;  // column pairs of each lane
+  const int lane = threadIdx.x & 31;
+  const int32_t* const table = a.pool.table + u.seq * a.pool.table_stride;
+  const int end = min((u.kb0 + u.blocks) * kRows, u.len);
+  for (int k0 = max(u.kb0 * kRows, u.first & ~31); k0 < end; k0 += 32) {
+    if (!u.edge(k0 & ~(kRows - 1))) continue;
+    int64_t at = 0;  // a key per lane: its row within the pool
+    if (k0 + lane < end) {
+      const int key = k0 + lane;
+      int page = table[key >> a.pool.page_shift];
+      if (page < 0 || page >= a.pool.num_pages) page = 0;  // as the copies take it
+      at = static_cast<int64_t>(page) * a.pool.page_stride + u.kvh * a.pool.head_stride +
+           (key & ((1 << a.pool.page_shift) - 1)) * a.pool.row_stride;
+    }
+    const int count = min(32, end - k0);
+    auto value = [&](int i, int c) -> uint32_t {  // bits that are not finite, of key k0 + i
+      const uint32_t w =
+          *reinterpret_cast<const uint32_t*>(a.v_pages + __shfl_sync(0xffffffffu, at, i) + 2 * (kWords * lane + c));
+      return w & not_finite<T>(w);
+    };
+    uint32_t keys = 0u;  // that have one
+#pragma unroll 8
+    for (int i = 0; i < count; ++i) {
+      uint32_t any = 0u;
+#pragma unroll
+      for (int c = 0; c < kWords; ++c) any |= value(i, c);
+      if (__any_sync(0xffffffffu, any != 0u)) keys |= 1u << i;
+    }
+    if (keys == 0u) continue;
+    for (uint32_t rows = __ballot_sync(0xffffffffu, live); rows != 0u; rows &= rows - 1) {
+      const int r = __ffs(rows) - 1;
+      const int r_lo = __shfl_sync(0xffffffffu, lo, r) - k0, r_hi = __shfl_sync(0xffffffffu, hi, r) - k0;
+      const int64_t r_dst = __shfl_sync(0xffffffffu, dst, r);
+      float4* const r_part = reinterpret_cast<float4*>(
+          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(part), r));
+      float2 sum[kWords] = {};
+      for (uint32_t k = keys; k != 0u; k &= k - 1) {
+        const int i = __ffs(k) - 1;
+        if (i < r_lo || i > r_hi) continue;
+#pragma unroll
+        for (int c = 0; c < kWords; ++c) {
+          const float2 x = Elem<T>::unpack(value(i, c));
+          sum[c].x += x.x, sum[c].y += x.y;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kWords; ++c) {
+        if (sum[c].x == 0.f && sum[c].y == 0.f) continue;
+        const int pair = kWords * lane + c;
+        if (part != nullptr) {
+          float2* const o = reinterpret_cast<float2*>(r_part + pair / 2 * 256) + pair % 2;
+          *o = make_float2(o->x + sum[c].x, o->y + sum[c].y);
+        } else {
+          uint32_t* const o = reinterpret_cast<uint32_t*>(a.out + r_dst) + pair;
+          const float2 x = Elem<T>::unpack(*o);
+          *o = Elem<T>::pack(x.x + sum[c].x, x.y + sum[c].y);
+        }
+      }
+    }
+  }
+}
+
 template <typename T>
 constexpr uint32_t idesc(int n) {
   // D fp32; A and B bf16 (bits 7, 10) or fp16 (none)
@@ -424,35 +521,36 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t* q_full = bars;
   uint64_t* q_empty = bars + 1;
-  uint64_t* v_raw = bars + 2;       // values with rows to be zeroed
-  uint64_t* mma_done = bars + 3;
-  uint64_t* s_full = bars + 4;      // [2]
-  uint64_t* p_full = bars + 6;      // [2]
-  uint64_t* o_full = bars + 8;      // [2]
-  uint64_t* u_full = bars + 10;     // [2] units announced by the TMA warp
-  uint64_t* u_empty = bars + 12;    // [2]
-  uint64_t* kv_full = bars + 14;    // [kStages]
+  uint64_t* mma_done = bars + 2;
+  uint64_t* s_full = bars + 3;      // [2]
+  uint64_t* p_full = bars + 5;      // [2]
+  uint64_t* o_full = bars + 7;      // [2]
+  uint64_t* u_full = bars + 9;      // [2] units announced by the TMA warp
+  uint64_t* u_empty = bars + 11;    // [2]
+  uint64_t* kv_full = bars + 13;    // [kStages]
   uint64_t* kv_empty = kv_full + kStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + kStages);
+  uint64_t* v_raw = kv_empty + kStages;  // [kStages] values of an edge block, unchecked
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_raw + kStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   Start* start = reinterpret_cast<Start*>(tmem_slot + 2);
   Unit* ring = reinterpret_cast<Unit*>(start + 1);  // [2]
-  static_assert((14 + 2 * kStages) * 8 + 8 + sizeof(Start) + 2 * sizeof(Unit) <= 512, "barrier area");
+  static_assert((13 + 3 * kStages) * 8 + 8 + sizeof(Start) + 2 * sizeof(Unit) <= 512, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 9) sm100::tmem_alloc(tmem_slot, kTmemCols);
   if (threadIdx.x == 352) {
-    for (int i = 0; i < 4; ++i) sm100::mbar_init(&bars[i], 1);
+    for (int i = 0; i < 3; ++i) sm100::mbar_init(&bars[i], 1);
     for (int i = 0; i < 2; ++i) {
       sm100::mbar_init(&s_full[i], 1);
       sm100::mbar_init(&p_full[i], 4);  // one arrival per softmax warp
       sm100::mbar_init(&o_full[i], 1);
       sm100::mbar_init(&u_full[i], 1);
-      sm100::mbar_init(&u_empty[i], 9);  // the softmax warps and the MMA warp
+      sm100::mbar_init(&u_empty[i], 10);  // the softmax, MMA and checking warps
     }
     for (int i = 0; i < kStages; ++i) {
       sm100::mbar_init(&kv_full[i], 1);
       sm100::mbar_init(&kv_empty[i], 1);
+      sm100::mbar_init(&v_raw[i], 1);
     }
     *abort_flag = 0;
     sm100::fence_mbar_init();
@@ -489,7 +587,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 8) {
       // ----------------------------------------------------------- TMA
-      uint32_t n_kv = 0, n_q = 0, n_raw = 0;
+      uint32_t n_kv = 0, n_q = 0;
+      uint32_t raw = 0, raw_ph = 0;  // by stage: its last copy is an unchecked one; their phases
       bool ok = true;
       const int page_rows = min(1 << a.pool.page_shift, kRows);  // rows per copy
       const int copies = kRows / page_rows * (D / 64);
@@ -534,33 +633,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
           }
           const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, held)) * page_rows * 128;
           const int in_page = key & ((1 << a.pool.page_shift) - 1);
-          const bool mend = key0 + kRows > len || key0 < lo;
+          const bool edge = u.edge(key0);
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             const uint32_t s = n_kv % kStages, ph = (n_kv / kStages) & 1;
             if (!(ok = wait(&kv_empty[s], ph ^ 1u, status, abort_flag))) break;
             uint8_t* dst = smem + L::kKV + s * L::kTile;
-            uint64_t* bar = kv == 1 && mend ? v_raw : &kv_full[s];
+            const bool check = kv == 1 && edge;
+            uint64_t* bar = check ? &v_raw[s] : &kv_full[s];
+            raw = (raw & ~(1u << s)) | (check ? 1u << s : 0u);
+            if (check) raw_ph ^= 1u << s;
             if (lane == 0) sm100::mbar_arrive_expect_tx(bar, bytes);
             __syncwarp();
             if (held)
               sm100::tma_load_4d(kv == 0 ? &map_k : &map_v, bar, dst + half * kBox + piece_row * 128,
                                  half * 64, in_page, kvh, page);
             ++n_kv;
-            if (kv == 1 && mend) {
-              if (!(ok = wait(v_raw, n_raw & 1, status, abort_flag))) break;
-              ++n_raw;
-              const int r0 = max(0, lo - key0), r1 = max(0, min(kRows, len - key0));
-              for (int k = lane; k < kRows * 8 * (D / 64); k += 32) {
-                const int r = (k >> 3) & (kRows - 1);
-                if (r < r0 || r >= r1)
-                  *reinterpret_cast<uint4*>(dst + (k >> 10) * kBox + r * 128 + (k & 7) * 16) =
-                      make_uint4(0, 0, 0, 0);
-              }
-              sm100::fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) sm100::mbar_arrive(&kv_full[s]);
-            }
           }
         }
       }
@@ -568,8 +656,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
       // timeout; otherwise every one of these has been waited for)
       if (!ok) {
         if (n_q > 0) wait(q_full, (n_q - 1) & 1, status, nullptr);
-        for (uint32_t i = 1; i <= kStages && i <= n_kv; ++i)
-          wait(&kv_full[(n_kv - i) % kStages], ((n_kv - i) / kStages) & 1, status, nullptr);
+        for (uint32_t i = 1; i <= kStages && i <= n_kv; ++i) {
+          const uint32_t n = n_kv - i, s = n % kStages;
+          if (raw >> s & 1) wait(&v_raw[s], (raw_ph >> s & 1) ^ 1u, status, nullptr);
+          else wait(&kv_full[s], (n / kStages) & 1, status, nullptr);
+        }
       }
     } else if (warp == 9) {
       // ---------------------------------------------------- MMA issuer
@@ -653,6 +744,61 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
       // every MMA completes before TMEM and shared memory go away
       commit(mma_done);
       wait(mma_done, 0, status, nullptr);
+    } else if (warp == 10) {
+      // ------------------------------------------- values of edge blocks
+      // A block that some row sees in part: zero weights meet its other values.
+      // Rows outside the sequence are zeroed, they may hold anything; values
+      // that are not finite are zeroed and added by the softmax warps to the rows
+      // that see them.  Beside the block's first product and softmax, which
+      // take longer.
+      uint32_t n_kv = 0, ph = 0;  // ph: phases of v_raw
+      bool ok = true;
+      for (uint32_t n = 0; ok && get(n); ++n) {
+        const Unit& u = ring[n & 1];
+        for (int j = u.blocks - 1; j >= 0; --j, n_kv += 2) {
+          const int key0 = (u.kb0 + j) * kRows;
+          if (!u.edge(key0)) continue;
+          const uint32_t s = (n_kv + 1) % kStages;
+          if (!(ok = wait(&v_raw[s], ph >> s & 1, status, abort_flag))) break;
+          ph ^= 1u << s;
+          uint4* const v = reinterpret_cast<uint4*>(smem + L::kKV + s * L::kTile);
+          const int r0 = max(0, u.first - key0), r1 = max(0, min(kRows, u.len - key0));
+          constexpr int kPieces = kRows * 8 * (D / 64);  // of 16 bytes, eight a row and box
+          if (r0 > 0 || r1 < kRows) {
+            for (int k = lane; k < kPieces; k += 32) {
+              const int r = k >> 3 & (kRows - 1);
+              if (r < r0 || r >= r1) v[k] = make_uint4(0, 0, 0, 0);
+            }
+            __syncwarp();
+          }
+          uint32_t acc[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 1
+          for (int k = lane; k < kPieces; k += 32 * 8) {
+            uint4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = v[k + 32 * i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              acc[0] = Elem<T>::probe(x[i].x, acc[0]), acc[1] = Elem<T>::probe(x[i].y, acc[1]);
+              acc[2] = Elem<T>::probe(x[i].z, acc[2]), acc[3] = Elem<T>::probe(x[i].w, acc[3]);
+            }
+          }
+          const uint32_t found = not_finite<T>(acc[0]) | not_finite<T>(acc[1]) |
+                                 not_finite<T>(acc[2]) | not_finite<T>(acc[3]);
+          if (__builtin_expect(__any_sync(0xffffffffu, found), 0)) {
+            for (int k = lane; k < kPieces; k += 32) {
+              const uint4 x = v[k];
+              v[k] = make_uint4(x.x & ~not_finite<T>(x.x), x.y & ~not_finite<T>(x.y),
+                                x.z & ~not_finite<T>(x.z), x.w & ~not_finite<T>(x.w));
+            }
+            if (lane == 0) ring[n & 1].odd = 1;  // before the arrival
+          }
+          sm100::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) sm100::mbar_arrive(&kv_full[s]);
+        }
+        done(n);
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -900,6 +1046,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
         else if (a.lse)
           a.lse[static_cast<int64_t>(u.token + local) * a.q_heads + head] = lse_of(m, l);
       }
+      if (__builtin_expect(u.odd, 0)) {
+        __syncwarp();  // behind the rows' stores
+        add_not_finite<T, D>(a, u, live, lo, hi, dst, whole ? nullptr : part);
+      }
       sm100::tc_fence_before();  // O is read before the next unit's first product
       done(n);
     }
@@ -1079,6 +1229,7 @@ LLMYB_API int32_t llmyb_paged_prefill(const llmyb_paged_args* x, void* stream) {
   if ((blocks + kUnitCost) * x->kv_heads >= 1ll << 26) return LLMYB_EUNSUPPORTED;
   PrefillArgs a;
   a.pool = paged_pool(x);
+  a.v_pages = static_cast<const uint16_t*>(x->v_pages);
   a.cu_q = x->cu_q, a.prefix = x->prefix, a.n_tokens = x->n_tokens, a.q_heads = x->q_heads;
   a.group = group, a.tile_tokens = kRows / group;
   a.window = x->window, a.scale = x->scale, a.softcap = x->softcap, a.slopes = x->slopes;

@@ -853,8 +853,8 @@ int32_t llmyb_paged_decode(const llmyb_paged_args* args, void* stream);
 /* The packed tokens of a call (their keys and values already in the pages):
  * scores as in llmyb_paged_decode, key j visible from position i if j <= i and
  * (window > 0) i - j < window, or (prefix, not together with a window)
- * j < prefix[b].  Rows that see no key give zeros.  Values of visible 128-key
- * blocks must be finite (rows outside the sequence may hold anything).
+ * j < prefix[b].  Rows that see no key give zeros.  Queries, keys and values
+ * that are not finite reach the rows that see them, and no other.
  * q_heads / kv_heads <= 128; kv_heads times the 128-key blocks that the table
  * can hold at most 2^26 (LLMYB_EUNSUPPORTED); scratch may be null where
  * scratch_bytes is 0. */

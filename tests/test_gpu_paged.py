@@ -1030,3 +1030,54 @@ def test_maximum_that_rises_late(cuda, dtype, pad, rise):
         tol = tol + max(lengths) * 2.0 ** -25 * np.abs(cache.v_ref).max()
     assert (np.abs(_np(out) - ref) <= tol).all()
     assert (np.abs(_np(lse) - l_ref) <= score + 2.0 ** -20 * np.abs(l_ref)).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,hq,kv,page,softcap,window,alibi,prefix,pad", [
+    (64, 4, 2, 16, 0, 0, False, None, 0), (128, 3, 1, 64, 0, 0, False, None, 30),
+    (64, 2, 1, 256, 20.0, 60, True, None, 0), (128, 4, 4, 16, 0, 100, True, None, 60),
+    (64, 5, 1, 32, 0, 0, True, [150, 0, 60], 40), (128, 2, 2, 128, 10.0, 0, False, [70, 280, 0], 0),
+    (128, 8, 1, 32, 5.0, 33, False, None, 20)])
+def test_values_that_are_not_finite_reach_only_their_readers(cuda, dtype, dim, hq, kv, page, softcap,
+                                                             window, alibi, prefix, pad):
+    """An infinity or a NaN in single columns of values that some rows of a block see and
+    others do not: in front of a row, behind its window, ahead of it within a prefix,
+    and before tokens that have no position.  The columns of rows that see one are not
+    finite; everything else is what it is with zeros in their place."""
+    from hybrid_llm_b200 import kernels
+    dt = DT[dtype]
+    new, context = [170, 40, 30], [30, 260, -12]
+    lengths = [a + b for a, b in zip(new, context)]
+    cache = Cache(lengths, kv, dim, page, dt, seed=72 + dim, pad=pad)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    spots = [(0, 77, 3, float("nan")), (0, 78, dim - 1, float("inf")), (0, 198, 8, -float("inf")),
+             (1, 250, 17, float("inf")), (1, 280, 40, float("nan")), (2, 0, 0, float("nan")),
+             (2, 17, dim - 2, float("inf"))]
+    see = np.zeros((cu[-1], dim), bool)      # columns that a row's keys make not finite
+    seq, pos = paged.positions(cu, lengths, cu[-1])
+    for b, key, col, what in spots:
+        at = cache.table[b, key // page], slice(None), key % page, col
+        cache.vd[at] = what
+        cache.v_ref[at] = 0.0
+        seen = (seq == b) & (pos >= 0) & ((key <= pos) & ((window == 0) | (pos - key < window)))
+        if prefix is not None:
+            seen |= (seq == b) & (pos >= 0) & (key < prefix[b])
+        see[seen, col] = True
+    g = torch.Generator().manual_seed(14)
+    q = torch.randn(cu[-1], hq, dim, generator=g).to(dt).cuda()
+    slopes = (torch.rand(hq, generator=g) * 0.2).cuda() if alibi else None
+    pre = None if prefix is None else torch.tensor(prefix, dtype=torch.int32, device="cuda")
+    lse = torch.empty(cu[-1], hq, device="cuda")
+    out = kernels.paged_prefill(q, cache.kd, cache.vd, cache.td, cache.ld,
+                                torch.from_numpy(cu.astype(np.int32)).cuda(), softcap=softcap,
+                                window=window, slopes=slopes, prefix=pre, lse=lse)
+    kernels.check_device_status()
+    there = torch.from_numpy(see).cuda()[:, None, :].expand(out.shape)
+    assert see.any() and not see.all(0).any()
+    assert not out[there].isfinite().any()
+    ref, _, _ = paged.attention(_np(q), cache.k_ref, cache.v_ref, cache.table, cache.lengths, cu,
+                                scale=dim ** -0.5, softcap=softcap, window=window, prefix=prefix,
+                                slopes=None if slopes is None else _np(slopes))
+    out = torch.where(there, torch.from_numpy(ref).cuda().to(dt), out)
+    _check(out, lse, cache, q, cu, dt, softcap=softcap, window=window, prefix=prefix,
+           slopes=None if slopes is None else _np(slopes))

@@ -212,8 +212,9 @@ inline int32_t paged_check(const llmyb_paged_args* a) {
       a->num_pages < 0 || a->table_width < 0)
     return LLMYB_EINVAL;
   if (a->n_tokens == 0 || a->batch == 0) return LLMYB_OK;
-  if (!a->q || !a->k_pages || !a->v_pages || !a->table || !a->lengths || !a->out ||
-      a->num_pages == 0)
+  // a table without columns has no address: its sequences are all empty
+  if (!a->q || !a->k_pages || !a->v_pages || (!a->table && a->table_width > 0) || !a->lengths ||
+      !a->out || a->num_pages == 0)
     return LLMYB_EINVAL;
   const int shift = page_shift_of(a->page_size);
   if (shift < 0 || (a->head_dim != 64 && a->head_dim != 128) ||

@@ -1081,3 +1081,25 @@ def test_values_that_are_not_finite_reach_only_their_readers(cuda, dtype, dim, h
     out = torch.where(there, torch.from_numpy(ref).cuda().to(dt), out)
     _check(out, lse, cache, q, cu, dt, softcap=softcap, window=window, prefix=prefix,
            slopes=None if slopes is None else _np(slopes))
+
+
+def test_tables_without_columns(cuda):
+    """No row has a page yet: outputs are zero, an append has nowhere to store."""
+    from hybrid_llm_b200 import kernels
+    cache = Cache([40, 9], 2, 64, 16, torch.bfloat16, seed=50)
+    x = torch.randn(2, 8, 64, device="cuda").bfloat16()
+    q, k, v = x[:, :4], x[:, 4:6], x[:, 6:]
+    cu = torch.arange(3, dtype=torch.int32, device="cuda")
+    table, none = cache.td[:, :0], torch.zeros_like(cache.ld)
+    before = cache.kd.clone()
+    for lengths in (none, cache.ld):  # attention counts what the table holds
+        for out in (kernels.paged_decode(q, cache.kd, cache.vd, table, lengths),
+                    kernels.paged_prefill(q, cache.kd, cache.vd, table, lengths, cu)):
+            assert (out == 0).all()
+    for packed in (None, cu):
+        assert (kernels.paged_append(q, k, v, cache.kd, cache.vd, table, none, cu_q=packed) == 0).all()
+    kernels.check_device_status()
+    kernels.paged_append(q, k, v, cache.kd, cache.vd, table, cache.ld)
+    with pytest.raises(RuntimeError, match="invalid argument"):
+        kernels.check_device_status()
+    assert torch.equal(cache.kd.view(torch.int16), before.view(torch.int16))

@@ -227,15 +227,16 @@ inline int32_t paged_check(const llmyb_paged_args* a) {
   return LLMYB_OK;
 }
 
-// Further for the attention calls.  Scores are formed in base 2 and, under a cap,
+// Further for the attention calls.  Scores are formed in base 2 (factors of log2 e,
+// below 1.5) and, under a cap,
 // as fractions of it: those factors must be numbers of fp32 (a cap so large or
 // small that they are not would make every score 0 or NaN).
 inline int32_t paged_check_scores(const llmyb_paged_args* a) {
   auto normal = [](float x) { return x >= FLT_MIN && x <= FLT_MAX; };
   if (a->q_heads % a->kv_heads != 0 || a->window < 0 || !normal(a->scale) ||
-      !normal(a->scale * kLog2e) || !(a->softcap >= 0.f))
+      !normal(1.5f * a->scale) || !(a->softcap >= 0.f))
     return LLMYB_EINVAL;
-  if (a->softcap > 0.f && (!normal(a->softcap * kLog2e) || !normal(a->scale / a->softcap) ||
+  if (a->softcap > 0.f && (!normal(1.5f * a->softcap) || !normal(a->scale / a->softcap) ||
                            !normal(2.f * a->scale / a->softcap)))
     return LLMYB_EINVAL;
   return LLMYB_OK;

@@ -209,7 +209,8 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(AppendArgs a,
 // Rounds per warp: one where that many warps do not fill the GPU's 64 per SM
 // (a token's latency counts), else eight, so that a token's lookups and angles
 // serve several heads: 14117 tokens of 16 + 2 x 16 heads, 347 MB, take 70 us
-// (0.76 of the copy rate).  Four rounds took 85 us where eight took 77; a CTA
+// in a graph of calls (0.76 of the copy rate; 74 us as single calls), with 72 %
+// of the issue slots busy.  Four rounds took 85 us where eight took 77; a CTA
 // per token with the angles in shared memory, 129 us.
 template <typename T, int DH, int kRounds>
 void launch(const AppendArgs& a, cudaStream_t s) {

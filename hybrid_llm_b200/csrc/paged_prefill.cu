@@ -938,7 +938,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
             }
           }
         };
-        auto weights = [&]() -> float {  // P = 2^(s - m) to TMEM, and its row sum
+        // P = 2^(s - m) to TMEM in the cache's type, the operand that the tensor
+        // cores take (each off by at most half a step, unbiased: errors against 64
+        // bits 0.0018-0.0024 of the output's size, its own rounding 0.0015-0.0017),
+        // and its row sum, unrounded
+        auto weights = [&]() -> float {
           const float base = m == -INFINITY ? 0.f : -m;
           const uint64_t sc2 = make2(sc, sc), base2 = make2(base, base);
           uint64_t rs[2] = {0ull, 0ull};

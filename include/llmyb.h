@@ -841,8 +841,8 @@ int32_t llmyb_paged_append(const llmyb_paged_args* args, void* stream);
 
 /* One token per sequence (n_tokens == batch; row b of q and out has position
  * lengths[b] - 1): out = softmax(s) v over its visible keys, s = scale q.k
- * (scale > 0), then softcap * tanh(s / softcap) if softcap > 0 (scale, softcap
- * and scale / softcap normal numbers of fp32, twice over: LLMYB_EINVAL), then
+ * (scale > 0), then softcap * tanh(s / softcap) if softcap > 0 (LLMYB_EINVAL
+ * where 1.5 scale, 1.5 softcap or 2 scale / softcap is no normal number of fp32), then
  * - slopes[h] * distance if slopes; window > 0: distance < window.  A sequence
  * of length 0 gives zeros.  lse: natural log of the sum of exp(s), -inf where
  * no key is visible.  scratch: scratch_bytes of the current device, not shared
@@ -855,8 +855,8 @@ int32_t llmyb_paged_decode(const llmyb_paged_args* args, void* stream);
  * (window > 0) i - j < window, or (prefix, not together with a window)
  * j < prefix[b].  Rows that see no key give zeros.  Queries, keys and values
  * that are not finite reach the rows that see them, and no other.
- * q_heads / kv_heads <= 128; kv_heads times the 128-key blocks that the table
- * can hold at most 2^26 (LLMYB_EUNSUPPORTED); scratch may be null where
+ * q_heads / kv_heads <= 128; kv_heads * (3 + the 128-key blocks that the table
+ * can hold) below 2^26 (LLMYB_EUNSUPPORTED); scratch may be null where
  * scratch_bytes is 0. */
 int64_t llmyb_paged_prefill_scratch_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                                           int32_t table_width, int32_t page_size);

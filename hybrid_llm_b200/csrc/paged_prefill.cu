@@ -33,9 +33,9 @@
 // (behind its end, or before the window; they may hold anything) are zeroed in
 // shared memory, and so are values that are not finite, which are added to the
 // outputs of the rows that see them (add_not_finite).  The check runs beside the
-// block's softmax: 1.6 % of a ragged batch under a window, where every fourth
-// block is an edge.  All waits are bounded; a timeout records LLMYB_ETIMEOUT and
-// every role unwinds.
+// block's softmax: 273 to 281 us for a ragged batch under a window, where about
+// three of a unit's nine blocks are such edges.  All waits are bounded; a timeout
+// records LLMYB_ETIMEOUT and every role unwinds.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -456,8 +456,8 @@ __device__ __forceinline__ void add_not_finite(const PrefillArgs& a, const Unit&
     }
     const int count = min(32, end - k0);
     auto value = [&](int i, int c) -> uint32_t {  // bits that are not finite, of key k0 + i
-      const uint32_t w =
-          *reinterpret_cast<const uint32_t*>(a.v_pages + __shfl_sync(0xffffffffu, at, i) + 2 * (kWords * lane + c));
+      const uint16_t* const row = a.v_pages + __shfl_sync(0xffffffffu, at, i);
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(row + 2 * (kWords * lane + c));
       return w & not_finite<T>(w);
     };
     uint32_t keys = 0u;  // that have one

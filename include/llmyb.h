@@ -798,8 +798,9 @@ int32_t llmyb_decode_persistent(const llmyb_pdecode* p, void* stream);
  * cu_q[b] .. cu_q[b + 1) are the last cu_q[b+1] - cu_q[b] positions of
  * sequence b; rows before cu_q[0] and behind cu_q[batch] may be read, but are
  * not used, and their outputs are left alone.  A page number outside
- * [0, num_pages) sets dev_status to LLMYB_EINVAL and is not accessed.  Outputs must not overlap themselves
- * nor inputs, except out == q in append.
+ * [0, num_pages) sets dev_status to LLMYB_EINVAL and is not accessed (prefill
+ * takes page 0 for it).  Outputs must not overlap themselves nor inputs, except
+ * out == q in append.
  *
  * The three calls take one argument block (host memory, read during the call);
  * fields that a call does not name are ignored. */
